@@ -245,6 +245,21 @@ int neat_tta_loss_fwd_bwd(const float* text, const float* pos, const float* inv,
 int neat_adamw_flat(float* p, const float* g, float* m, float* v, long n, double lr, double beta1,
                     double beta2, double eps, double wd, int step, void* stream);
 
+/* The same rule for `count` tensors that stay where they are, in one launch per 96 tensors, moments in 32 or in 8 bits.
+ * p, g, n, state_block, step are HOST arrays of `count` entries, read before the call returns; p[i] / g[i] are device
+ * addresses of n[i] elements of `dtype` (NEAT_F32 / NEAT_BF16, parameters and gradients alike), aligned to their elements
+ * only; n[i] == 0 is skipped; step[i] >= 1 counts the tensor's own steps, this one included.
+ * The moments of tensor i start at block state_block[i] of m and v and fill ceil(n[i] / 256) blocks of 256 elements (the
+ * last one padded: the padding must be zero at first and stays zero).  state_bits == 32: m, v f32 [blocks, 256], scales
+ * unused (may be NULL).  state_bits == 8: m, v u8 [blocks, 256] hold e4m3 codes, m_scale, v_scale f32 [blocks] a power of two
+ * each; moment 1 = code * m_scale, SQUARE ROOT of moment 2 = code * v_scale.  The step uses the moments before they are rounded.
+ * A value that is not finite becomes a NaN code of its own and leaves its block's scale alone.  Tensors and blocks of one
+ * call must not overlap.  The step counts are host values: a captured launch replays them as they were. */
+enum { NEAT_F32 = 0, NEAT_BF16 = 1 };   /* element types */
+int neat_adamw_multi(int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* state_block,
+                     const int32_t* step, int dtype, void* m, void* v, float* m_scale, float* v_scale, int state_bits,
+                     double lr, double beta1, double beta2, double eps, double wd, void* stream);
+
 /* ---- retrieval scoring, evaluation/retrieval.py:280-301 ---- */
 /* Row-wise top-k of a strided f32 matrix (element (r,c) at scores[r*ld_row + c*ld_col]; one of the
  * strides must be 1 -> accepts scores and scores.T).  idx i32 [R,k] descending, ties -> lowest index;

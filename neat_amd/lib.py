@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NEAT_HIP_LIB") or os.path.join(_HERE, "libneat_hip.so")
 
 EPI_BF16, EPI_BIAS_BF16, EPI_BIAS_RES_F32, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_F32 = range(6)
+DT_F32, DT_BF16 = range(2)
 
 _P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_double
 
@@ -57,6 +58,7 @@ SIGNATURES = {
     "neat_loss_ws_floats": (_L, [_I, _I]),
     "neat_tta_loss_fwd_bwd": (_I, [_P, _P, _P, _P, _P, _F, _F, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "neat_adamw_flat": (_I, [_P, _P, _P, _P, _L, _D, _D, _D, _D, _D, _I, _P]),
+    "neat_adamw_multi": (_I, [_I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _D, _D, _D, _D, _D, _P]),
     "neat_topk_ws_bytes": (_L, [_I, _I, _I]),
     "neat_topk_rows": (_I, [_P, _L, _L, _I, _I, _I, _P, _P, _P, _P]),
     "neat_recall_from_topk": (_I, [_P, _P, _L, _L, _I, _I, _I, _P, _P]),

@@ -6,6 +6,7 @@ raise RuntimeError on any failure -- there is no eager fallback.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 from typing import Optional, Tuple
 
@@ -516,6 +517,78 @@ def tta_loss_fwd_bwd(text, pos, inv, text_all, coarse_all, T1, T2, row0=0):
 def adamw_flat(p, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0):
     lib.call("neat_adamw_flat", _p(p, f32, "p"), _p(g, f32, "g"), _p(m, f32, "m"), _p(v, f32, "v"), p.numel(), float(lr),
              float(beta1), float(beta2), float(eps), float(wd), int(step), _stream())
+
+
+class _OnDevice:
+    """Makes the tensors' device current for a launch where it is not (the library launches on the current device)."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == _device_index() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _device_index() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
+ADAMW_BLOCK = 256            # elements of one tensor that share a block of moments (and, in 8 bits, a scale)
+_DTYPES = {f32: lib.DT_F32, bf16: lib.DT_BF16}
+
+
+def adamw_multi(params, grads, state_blocks, steps, m, v, m_scale=None, v_scale=None, lr=1e-3, beta1=0.9, beta2=0.999,
+                eps=1e-8, wd=0.0):
+    """One AdamW step over a list of tensors of one dtype (float32 or bfloat16) that stay where they are, in one launch
+    per 96 tensors (neat_adamw_multi; ``optim.MultiTensorAdamW`` keeps the moments and calls this).  Tensor i's moments
+    start at block ``state_blocks[i]`` of m / v [blocks, 256]: float32, or uint8 e4m3 codes with the scales m_scale /
+    v_scale [blocks] (v then holds the square root).  ``steps[i]`` >= 1 counts tensor i's steps, this one included.
+    The step counts and rates are host values, so a call inside a graph capture is refused."""
+    count = len(params)
+    if not (len(grads) == len(state_blocks) == len(steps) == count):
+        raise RuntimeError("adamw_multi: one gradient, state block and step count per parameter expected")
+    if count == 0:
+        return
+    bits = 8 if m.dtype == torch.uint8 else 32
+    if m.dtype != (torch.uint8 if bits == 8 else f32) or v.dtype != m.dtype or m.shape != v.shape or m.dim() != 2 \
+            or m.shape[1] != ADAMW_BLOCK:
+        raise RuntimeError("adamw_multi: m and v must be float32 or uint8 [blocks, 256], alike")
+    dtype, device = params[0].dtype, params[0].device
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"adamw_multi: parameters must be float32 or bfloat16, got {dtype}")
+    if {t.dtype for t in params} != {dtype} or {t.dtype for t in grads} != {dtype}:
+        raise RuntimeError(f"adamw_multi: parameters and gradients must all be {dtype}")
+    if {t.device for t in params} != {device} or {t.device for t in grads} != {device} or m.device != device \
+            or v.device != device:
+        raise RuntimeError("adamw_multi: all tensors must be on one device")
+    if not all(t.is_contiguous() for t in params) or not all(t.is_contiguous() for t in grads):
+        raise RuntimeError("adamw_multi: parameters and gradients must be contiguous")
+    sizes = [t.numel() for t in params]
+    if [t.numel() for t in grads] != sizes:
+        raise RuntimeError("adamw_multi: a gradient differs in size from its parameter")
+    blocks = m.shape[0]
+    if any(b < 0 or b + (n + ADAMW_BLOCK - 1) // ADAMW_BLOCK > blocks for b, n in zip(state_blocks, sizes)):
+        raise RuntimeError("adamw_multi: a tensor's moments lie outside m / v")
+    if bits == 8:
+        for t, nm in ((m_scale, "m_scale"), (v_scale, "v_scale")):
+            if t is None or tuple(t.shape) != (blocks,) or t.device != device:
+                raise RuntimeError(f"adamw_multi: {nm} must be float32 [{blocks}] on the parameters' device")
+    if not device.type == "cuda":
+        raise RuntimeError("adamw_multi: expected GPU tensors (libneat_hip has no CPU path)")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_multi: the step counts are host values that a graph would replay unchanged: "
+                           "capture the backward pass and step outside the graph")
+    ptrs, longs, ints = ctypes.c_void_p * count, ctypes.c_int64 * count, ctypes.c_int32 * count
+    with _OnDevice(device):
+        lib.call("neat_adamw_multi", count, ptrs(*[t.data_ptr() for t in params]), ptrs(*[t.data_ptr() for t in grads]),
+                 longs(*sizes), longs(*state_blocks), ints(*steps), _DTYPES[dtype], _p(m), _p(v),
+                 _p(m_scale, f32, "m_scale"), _p(v_scale, f32, "v_scale"), bits, float(lr), float(beta1), float(beta2),
+                 float(eps), float(wd), _stream())
 
 
 # ---- retrieval ----

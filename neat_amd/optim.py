@@ -5,6 +5,9 @@ weight_decay = tta_wd, betas (0.9, 0.999), eps 1e-8; state persists across batch
 parameter tensors are re-pointed at construction to views of one flat fp32 buffer, their ``.grad`` to
 views of a flat gradient buffer, so ``step()`` is a single ``neat_adamw_flat`` launch instead of 48
 small ones and a data-parallel gradient all-reduce is one collective over ``flat_grad``.
+
+``MultiTensorAdamW`` applies the same rule to any number of tensors that stay where they are -- float32 or bfloat16, several
+parameter groups, gradients that come and go -- with moments in 32 or in 8 bits (``neat_adamw_multi``).
 """
 from __future__ import annotations
 
@@ -61,3 +64,123 @@ class AdamW(torch.optim.Optimizer):
     def zero_grad(self, set_to_none: bool = False):
         # gradients are views of flat_grad and must stay attached; the backward overwrites them
         self.flat_grad.zero_()
+
+
+class MultiTensorAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` over float32 / bfloat16 parameters of any sizes, one launch per 96 tensors.
+
+    ``state_bits=32``: the moments are ``exp_avg`` and ``exp_avg_sq``, float32 [blocks, 256]; every parameter owns
+    ceil(numel / 256) blocks, in parameter order.  ``state_bits=8``: ``exp_avg`` and ``exp_avg_root`` (the SQUARE ROOT of
+    the second moment) are e4m3 numbers [blocks, 256], each block times its power of two ``exp_avg_scale`` /
+    ``exp_avg_root_scale`` [blocks]: 2 bytes an element instead of 8.  ``moments(p)`` gives one parameter's as it would be
+    in 32 bits.  A parameter whose ``.grad`` is None is left alone and its step count stays (as in torch)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"MultiTensorAdamW: state_bits must be 32 or 8, got {state_bits}")
+        self._ready = False
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        for g in self.param_groups:
+            self._check_group(g)
+        ps = [p for g in self.param_groups for p in g["params"]]
+        if not ps:
+            raise ValueError("MultiTensorAdamW: empty parameter list")
+        if len({id(p) for p in ps}) != len(ps):
+            raise ValueError("MultiTensorAdamW: a parameter is listed twice")
+        self.device = ps[0].device
+        if self.device.type != "cuda" or any(p.device != self.device for p in ps):
+            raise RuntimeError("MultiTensorAdamW: parameters must be on one GPU")
+        for p in ps:
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                raise RuntimeError(f"MultiTensorAdamW: parameters must be float32 or bfloat16, got {p.dtype}")
+            if not p.is_contiguous():
+                raise RuntimeError("MultiTensorAdamW: parameters must be contiguous")
+        self.state_bits = state_bits
+        blocks, self._first, self._numel, self._steps = 0, {}, {}, {}
+        for p in ps:
+            self._first[p], self._numel[p], self._steps[p] = blocks, p.numel(), 0
+            blocks += -(-p.numel() // ops.ADAMW_BLOCK)
+        dt = torch.uint8 if state_bits == 8 else torch.float32
+        self._m = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
+        self._v = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
+        self._ms = torch.ones(blocks, device=self.device) if state_bits == 8 else None
+        self._vs = torch.ones(blocks, device=self.device) if state_bits == 8 else None
+        # e4m3 views of the codes (the same memory)
+        self.exp_avg = self._m.view(torch.float8_e4m3fn) if state_bits == 8 else self._m
+        if state_bits == 8:
+            self.exp_avg_root, self.exp_avg_scale, self.exp_avg_root_scale = self._v.view(torch.float8_e4m3fn), self._ms, self._vs
+        else:
+            self.exp_avg_sq = self._v
+        self._ready = True
+
+    @staticmethod
+    def _check_group(g):
+        b1, b2 = g["betas"]
+        if not 0.0 <= b1 < 1.0 or not 0.0 <= b2 < 1.0:
+            raise ValueError(f"MultiTensorAdamW: betas must lie in [0, 1), got {g['betas']}")
+        if g["lr"] < 0.0 or g["eps"] < 0.0 or g["weight_decay"] < 0.0:
+            raise ValueError("MultiTensorAdamW: lr, eps and weight_decay must not be negative")
+
+    def add_param_group(self, group):
+        if getattr(self, "_ready", False):
+            raise RuntimeError("MultiTensorAdamW: the moments are laid out when it is built; pass all groups then")
+        super().add_param_group(group)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = []
+        for group in self.param_groups:
+            by_dtype = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    by_dtype.setdefault(p.dtype, []).append(p)
+            for ps in by_dtype.values():
+                grads = [p.grad for p in ps]
+                if any(g.layout != torch.strided for g in grads):
+                    raise RuntimeError("MultiTensorAdamW: sparse gradients are not supported")
+                if [p.numel() for p in ps] != [self._numel[p] for p in ps]:
+                    raise RuntimeError("MultiTensorAdamW: a parameter changed its size after the optimizer was built")
+                calls.append((group, ps, [g.contiguous() for g in grads]))
+        for group, ps, grads in calls:
+            b1, b2 = group["betas"]
+            ops.adamw_multi(ps, grads, [self._first[p] for p in ps], [self._steps[p] + 1 for p in ps], self._m,
+                            self._v, self._ms, self._vs, group["lr"], b1, b2, group["eps"], group["weight_decay"])
+            for p in ps:
+                self._steps[p] += 1
+        return loss
+
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of one parameter in float32, in its shape, and its step count."""
+        if p not in self._first:
+            raise ValueError("MultiTensorAdamW: not one of this optimizer's parameters")
+        n, lo = self._numel[p], self._first[p]
+        rows = slice(lo, lo - (-n // ops.ADAMW_BLOCK))
+        m, v = self.exp_avg[rows].float(), (self.exp_avg_root if self.state_bits == 8 else self._v)[rows].float()
+        if self.state_bits == 8:
+            m, v = m * self._ms[rows, None], (v * self._vs[rows, None]) ** 2
+        return m.reshape(-1)[:n].view(p.shape), v.reshape(-1)[:n].view(p.shape), self._steps[p]
+
+    def _buffers(self):
+        return [t for t in (self._m, self._v, self._ms, self._vs) if t is not None]
+
+    def state_dict(self):
+        d = super().state_dict()
+        ps = [p for g in self.param_groups for p in g["params"]]
+        d["state"] = {"state_bits": self.state_bits, "numels": [self._numel[p] for p in ps],
+                      "steps": [self._steps[p] for p in ps], "buffers": self._buffers()}
+        return d
+
+    def load_state_dict(self, state_dict):
+        st = state_dict["state"]
+        ps = [p for g in self.param_groups for p in g["params"]]
+        if st.get("state_bits") != self.state_bits or st["numels"] != [self._numel[p] for p in ps]:
+            raise ValueError("MultiTensorAdamW: the state belongs to other parameters or another state_bits")
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        for dst, src in zip(self._buffers(), st["buffers"]):
+            dst.copy_(src)
+        for p, k in zip(ps, st["steps"]):
+            self._steps[p] = int(k)
