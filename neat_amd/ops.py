@@ -548,47 +548,60 @@ def adamw_multi(params, grads, state_blocks, steps, m, v, m_scale=None, v_scale=
     per 96 tensors (neat_adamw_multi; ``optim.MultiTensorAdamW`` keeps the moments and calls this).  Tensor i's moments
     start at block ``state_blocks[i]`` of m / v [blocks, 256]: float32, or uint8 e4m3 codes with the scales m_scale /
     v_scale [blocks] (v then holds the square root).  ``steps[i]`` >= 1 counts tensor i's steps, this one included.
-    The step counts and rates are host values, so a call inside a graph capture is refused."""
+    Tensors, and blocks, must not overlap.  The step counts and rates are host values, so a call inside a graph capture is
+    refused."""
     count = len(params)
     if not (len(grads) == len(state_blocks) == len(steps) == count):
         raise RuntimeError("adamw_multi: one gradient, state block and step count per parameter expected")
     if count == 0:
         return
-    bits = 8 if m.dtype == torch.uint8 else 32
-    if m.dtype != (torch.uint8 if bits == 8 else f32) or v.dtype != m.dtype or m.shape != v.shape or m.dim() != 2 \
+    if m.dtype not in (torch.uint8, f32) or v.dtype != m.dtype or m.shape != v.shape or m.dim() != 2 \
             or m.shape[1] != ADAMW_BLOCK:
         raise RuntimeError("adamw_multi: m and v must be float32 or uint8 [blocks, 256], alike")
-    dtype, device = params[0].dtype, params[0].device
+    device = params[0].device
+    if v.device != device or m.device != device:
+        raise RuntimeError("adamw_multi: all tensors must be on one device")
+    sizes = [t.numel() for t in params]
+    blocks = m.shape[0]
+    if any(b < 0 or b + (n + ADAMW_BLOCK - 1) // ADAMW_BLOCK > blocks for b, n in zip(state_blocks, sizes)):
+        raise RuntimeError("adamw_multi: a tensor's moments lie outside m / v")
+    if m.dtype == torch.uint8:
+        for t, nm in ((m_scale, "m_scale"), (v_scale, "v_scale")):
+            if t is None or tuple(t.shape) != (blocks,) or t.device != device:
+                raise RuntimeError(f"adamw_multi: {nm} must be float32 [{blocks}] on the parameters' device")
+    _adamw_multi(params, grads, sizes, (ctypes.c_int64 * count)(*sizes), (ctypes.c_int64 * count)(*state_blocks), steps, m, v,
+                 m_scale, v_scale, lr, beta1, beta2, eps, wd)
+
+
+def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd):
+    """The launch behind adamw_multi, for moments that are known to hold tensors of ``sizes`` at ``blocks_c``; it looks at
+    what a caller can change between two steps (every check is one pass over the list: 48 small tensors cost the host more
+    than the GPU)."""
+    count, first = len(params), params[0]
+    dtype, index = first.dtype, first.get_device()
     if dtype not in _DTYPES:
         raise RuntimeError(f"adamw_multi: parameters must be float32 or bfloat16, got {dtype}")
     if {t.dtype for t in params} != {dtype} or {t.dtype for t in grads} != {dtype}:
         raise RuntimeError(f"adamw_multi: parameters and gradients must all be {dtype}")
-    if {t.device for t in params} != {device} or {t.device for t in grads} != {device} or m.device != device \
-            or v.device != device:
+    if not all([t.is_contiguous() for t in params]):
+        raise RuntimeError("adamw_multi: parameters must be contiguous")
+    if not all([t.is_contiguous() for t in grads]):
+        grads = [t.contiguous() for t in grads]
+    if [t.numel() for t in params] != sizes or [t.numel() for t in grads] != sizes:
+        raise RuntimeError("adamw_multi: a gradient or parameter differs in size from what the moments were laid out for")
+    if {t.get_device() for t in params} != {index} or {t.get_device() for t in grads} != {index}:
         raise RuntimeError("adamw_multi: all tensors must be on one device")
-    if not all(t.is_contiguous() for t in params) or not all(t.is_contiguous() for t in grads):
-        raise RuntimeError("adamw_multi: parameters and gradients must be contiguous")
-    sizes = [t.numel() for t in params]
-    if [t.numel() for t in grads] != sizes:
-        raise RuntimeError("adamw_multi: a gradient differs in size from its parameter")
-    blocks = m.shape[0]
-    if any(b < 0 or b + (n + ADAMW_BLOCK - 1) // ADAMW_BLOCK > blocks for b, n in zip(state_blocks, sizes)):
-        raise RuntimeError("adamw_multi: a tensor's moments lie outside m / v")
-    if bits == 8:
-        for t, nm in ((m_scale, "m_scale"), (v_scale, "v_scale")):
-            if t is None or tuple(t.shape) != (blocks,) or t.device != device:
-                raise RuntimeError(f"adamw_multi: {nm} must be float32 [{blocks}] on the parameters' device")
-    if not device.type == "cuda":
+    if index < 0:
         raise RuntimeError("adamw_multi: expected GPU tensors (libneat_hip has no CPU path)")
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_multi: the step counts are host values that a graph would replay unchanged: "
                            "capture the backward pass and step outside the graph")
-    ptrs, longs, ints = ctypes.c_void_p * count, ctypes.c_int64 * count, ctypes.c_int32 * count
-    with _OnDevice(device):
+    ptrs = ctypes.c_void_p * count
+    with _OnDevice(first.device):
         lib.call("neat_adamw_multi", count, ptrs(*[t.data_ptr() for t in params]), ptrs(*[t.data_ptr() for t in grads]),
-                 longs(*sizes), longs(*state_blocks), ints(*steps), _DTYPES[dtype], _p(m), _p(v),
-                 _p(m_scale, f32, "m_scale"), _p(v_scale, f32, "v_scale"), bits, float(lr), float(beta1), float(beta2),
-                 float(eps), float(wd), _stream())
+                 sizes_c, blocks_c, (ctypes.c_int32 * count)(*steps), _DTYPES[dtype], _p(m), _p(v),
+                 _p(m_scale, f32, "m_scale"), _p(v_scale, f32, "v_scale"), 8 if m.dtype == torch.uint8 else 32, lr, beta1,
+                 beta2, eps, wd, _stream())
 
 
 # ---- retrieval ----

@@ -11,6 +11,8 @@ parameter groups, gradients that come and go -- with moments in 32 or in 8 bits 
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import ops
@@ -96,10 +98,17 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             if not p.is_contiguous():
                 raise RuntimeError("MultiTensorAdamW: parameters must be contiguous")
         self.state_bits = state_bits
-        blocks, self._first, self._numel, self._steps = 0, {}, {}, {}
+        blocks, self._first, self._numel = 0, {}, {}
         for p in ps:
-            self._first[p], self._numel[p], self._steps[p] = blocks, p.numel(), 0
+            self._first[p], self._numel[p] = blocks, p.numel()
             blocks += -(-p.numel() // ops.ADAMW_BLOCK)
+        # per group and type, what one call of the library updates: [group, parameters, their layout, their step counts]
+        self._lists = []
+        for i, g in enumerate(self.param_groups):
+            for dt in (torch.float32, torch.bfloat16):
+                sub = [p for p in g["params"] if p.dtype == dt]
+                if sub:
+                    self._lists.append([i, sub, self._layout(sub), [0] * len(sub)])
         dt = torch.uint8 if state_bits == 8 else torch.float32
         self._m = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
         self._v = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
@@ -112,6 +121,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         else:
             self.exp_avg_sq = self._v
         self._ready = True
+
+    def _layout(self, ps):
+        """(sizes, the same as a C array, first blocks of the moments as a C array)."""
+        sizes = [self._numel[p] for p in ps]
+        longs = ctypes.c_int64 * len(ps)
+        return sizes, longs(*sizes), longs(*[self._first[p] for p in ps])
 
     @staticmethod
     def _check_group(g):
@@ -132,26 +147,29 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls = []
-        for group in self.param_groups:
-            by_dtype = {}
-            for p in group["params"]:
-                if p.grad is not None:
-                    by_dtype.setdefault(p.dtype, []).append(p)
-            for ps in by_dtype.values():
-                grads = [p.grad for p in ps]
-                if any(g.layout != torch.strided for g in grads):
-                    raise RuntimeError("MultiTensorAdamW: sparse gradients are not supported")
-                if [p.numel() for p in ps] != [self._numel[p] for p in ps]:
-                    raise RuntimeError("MultiTensorAdamW: a parameter changed its size after the optimizer was built")
-                calls.append((group, ps, [g.contiguous() for g in grads]))
-        for group, ps, grads in calls:
+        for i, ps, layout, steps in self._lists:
+            grads = [p.grad for p in ps]
+            at = None
+            if any([g is None for g in grads]):
+                at = [k for k, g in enumerate(grads) if g is not None]
+                if not at:
+                    continue
+                ps, grads = [ps[k] for k in at], [grads[k] for k in at]
+                layout = self._layout(ps)
+            now = [k + 1 for k in (steps if at is None else [steps[j] for j in at])]
+            group = self.param_groups[i]
             b1, b2 = group["betas"]
-            ops.adamw_multi(ps, grads, [self._first[p] for p in ps], [self._steps[p] + 1 for p in ps], self._m,
-                            self._v, self._ms, self._vs, group["lr"], b1, b2, group["eps"], group["weight_decay"])
-            for p in ps:
-                self._steps[p] += 1
+            ops._adamw_multi(ps, grads, *layout, now, self._m, self._v, self._ms, self._vs, float(group["lr"]), float(b1),
+                             float(b2), float(group["eps"]), float(group["weight_decay"]))
+            if at is None:
+                steps[:] = now
+            else:
+                for j, k in zip(at, now):
+                    steps[j] = k
         return loss
+
+    def _step_counts(self):
+        return {p: k for _, ps, _, steps in self._lists for p, k in zip(ps, steps)}
 
     def moments(self, p):
         """(exp_avg, exp_avg_sq) of one parameter in float32, in its shape, and its step count."""
@@ -162,25 +180,25 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         m, v = self.exp_avg[rows].float(), (self.exp_avg_root if self.state_bits == 8 else self._v)[rows].float()
         if self.state_bits == 8:
             m, v = m * self._ms[rows, None], (v * self._vs[rows, None]) ** 2
-        return m.reshape(-1)[:n].view(p.shape), v.reshape(-1)[:n].view(p.shape), self._steps[p]
+        return m.reshape(-1)[:n].view(p.shape), v.reshape(-1)[:n].view(p.shape), self._step_counts()[p]
 
     def _buffers(self):
         return [t for t in (self._m, self._v, self._ms, self._vs) if t is not None]
 
     def state_dict(self):
         d = super().state_dict()
-        ps = [p for g in self.param_groups for p in g["params"]]
-        d["state"] = {"state_bits": self.state_bits, "numels": [self._numel[p] for p in ps],
-                      "steps": [self._steps[p] for p in ps], "buffers": self._buffers()}
+        ps, steps = list(self._numel), self._step_counts()
+        d["state"] = {"state_bits": self.state_bits, "numels": [self._numel[p] for p in ps], "steps": [steps[p] for p in ps],
+                      "buffers": self._buffers()}
         return d
 
     def load_state_dict(self, state_dict):
-        st = state_dict["state"]
-        ps = [p for g in self.param_groups for p in g["params"]]
+        st, ps = state_dict["state"], list(self._numel)
         if st.get("state_bits") != self.state_bits or st["numels"] != [self._numel[p] for p in ps]:
             raise ValueError("MultiTensorAdamW: the state belongs to other parameters or another state_bits")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for dst, src in zip(self._buffers(), st["buffers"]):
             dst.copy_(src)
-        for p, k in zip(ps, st["steps"]):
-            self._steps[p] = int(k)
+        steps = dict(zip(ps, st["steps"]))
+        for _, sub, _, held in self._lists:
+            held[:] = [int(steps[p]) for p in sub]
