@@ -10,7 +10,8 @@
 // it, 448 being e4m3's largest.  A root above zero never becomes zero (it is held at the smallest code): a second moment lost
 // beside a first moment that is not would blow the next step up.  The step itself uses the moments before they are rounded.
 //
-// Mapping: four contiguous elements a lane (16 B of fp32), a block of 256 elements per wave instruction, four blocks a wave.  Tensor addresses travel as kernel arguments (96 tensors a launch): no table in device memory, so no copy to order
+// Mapping: a wave takes four blocks, a row of 16 lanes each, four times four contiguous elements a lane: whole 256-B runs of
+// fp32 per row and load, one reduction for four blocks, and all loads of a unit in flight together.  Tensor addresses travel as kernel arguments (96 tensors a launch): no table in device memory, so no copy to order
 // behind other work and none to keep alive.
 #include <math.h>
 
@@ -18,9 +19,9 @@
 
 namespace neat {
 
-constexpr int AW_BLOCK = 256;       // elements per block of moments = 64 lanes x 4
+constexpr int AW_BLOCK = 256;       // elements per block of moments = 16 lanes x 16
 constexpr int AW_WAVES = 4;
-constexpr int AW_UNIT = 4;          // blocks a wave takes, their loads in flight together
+constexpr int AW_UNIT = 4;          // blocks a wave takes, one for each row of 16 lanes
 constexpr int AW_TENSORS = 96;      // 96 x 40 B of kernel arguments beside the launch's own ~80 B; 4 096 B is the limit
 
 struct AwTensor {
@@ -71,20 +72,35 @@ template <> struct AwIo<bf16_t> {
     static __device__ __forceinline__ void store1(void* p, long i, float x) { static_cast<bf16_t*>(p)[i] = f2bf(x); }
 };
 
-// 2^e with the largest finite |x| of a block in (224, 448] x 2^e; 2^-126 for a block of zeros
-__device__ __forceinline__ int aw_exponent(float largest) {
-    const uint32_t u = __float_as_uint(largest);
-    const int e = (int)(u >> 23) - 126 - 9 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);   // mantissa above 1.75: one more
+// Largest x <= 448 x 2^e fixes e; both as bits, x >= 0 and normal or zero (a block of zeros takes the smallest power).
+// For a first moment |m|: one more where the mantissa is above 448 / 256 = 1.75.
+__device__ __forceinline__ int aw_exponent(uint32_t u) {
+    const int e = (int)(u >> 23) - 135 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
+}
+// The same for a root, from the second moment itself: sqrt(v) <= 448 x 2^e  <=>  v <= 448^2 x 4^e, 448^2 = 1.53125 x 2^17
+// (a rounded root lies on the same side: the float behind 448^2 x 4^e has a root above 448 x 2^e by more than half a step).
+__device__ __forceinline__ int aw_root_exponent(uint32_t u) {
+    const int e = ((int)(u >> 23) - 143 + ((u & 0x7fffffu) > 0x440000u ? 1 : 0)) >> 1;
+    return u == 0u ? -126 : e;
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// four numbers to e4m3, nearest even; what is not finite becomes NaN
+// largest of a row of 16 lanes, on the vector ALU alone
+__device__ __forceinline__ uint32_t aw_row_max(uint32_t v) {
+    uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);       // lane ^ 1
+    v = o > v ? o : v;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);                // lane ^ 2
+    v = o > v ? o : v;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);               // half a row mirrored
+    v = o > v ? o : v;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true);               // the row mirrored
+    return o > v ? o : v;
+}
+
+// four numbers to e4m3, nearest even
 __device__ __forceinline__ uint32_t to_e4m3(f32x4 q) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (!(fabsf(q[j]) < INFINITY)) q[j] = NAN;
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
 }
 __device__ __forceinline__ f32x4 from_e4m3(uint32_t w) {
@@ -92,115 +108,164 @@ __device__ __forceinline__ f32x4 from_e4m3(uint32_t w) {
     return f32x4{a[0], a[1], b[0], b[1]};
 }
 
-// largest of a wave, on the vector ALU alone: four steps inside rows of 16 lanes, then across the rows
-__device__ __forceinline__ float aw_wave_max(float v) {
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true)));     // lane ^ 1
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true)));     // lane ^ 2
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true)));    // half row mirrored
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xf, 0xf, true)));    // row mirrored
-    const float a = fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0)),
-                          __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16)));
-    const float b = fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32)),
-                          __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48)));
-    return fmaxf(a, b);
+// A wave's moments as they are held, between its loads and its stores: four groups of four elements a lane.
+template <bool SMALL> struct AwHeld;
+template <> struct AwHeld<false> { f32x4 m[4], v[4]; };
+template <> struct AwHeld<true> { uint32_t m[4], v[4]; float ms, vs; };
+
+// the scales of a row's new moments, and the moments as multiples of them
+__device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 (&v)[4], f32x4 (&r)[4], const f32x4 (&g)[4],
+                                          bool from_zero, const AwLaunch& a) {
+    constexpr uint32_t INF = 0x7f800000u, TINY = 0x00800000u;
+    uint32_t mm = 0, vm = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {                   // as bits: what is not finite is larger than all that is
+            const uint32_t um = __float_as_uint(m[k][j]) & 0x7fffffffu, uv = __float_as_uint(v[k][j]) & 0x7fffffffu;
+            mm = um > mm ? um : mm;
+            vm = uv > vm ? uv : vm;
+        }
+    mm = aw_row_max(mm);
+    vm = aw_row_max(vm);
+    if (__any(mm >= INF || vm >= INF)) {                // what is not finite does not set the scale of its neighbours
+        asm volatile("");                               // rare: to be branched around, not computed along
+        mm = vm = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t um = __float_as_uint(m[k][j]) & 0x7fffffffu, uv = __float_as_uint(v[k][j]) & 0x7fffffffu;
+                mm = um > mm && um < INF ? um : mm;
+                vm = uv > vm && uv < INF ? uv : vm;
+                if (um >= INF) m[k][j] = NAN;
+                if (uv >= INF) r[k][j] = INFINITY;      // no e4m3 number: becomes NaN
+            }
+        mm = aw_row_max(mm);
+        vm = aw_row_max(vm);
+    }
+    const int me = aw_exponent(mm);
+    int re = aw_root_exponent(vm);
+    if (__any(vm != 0u && vm < TINY)) re = vm < TINY ? aw_exponent(__float_as_uint(sqrtf(__uint_as_float(vm)))) : re;
+    const float mi = pow2i(-me), ri = pow2i(-re);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[k][j] *= mi;
+            // above zero: at least the smallest code.  The median of three is that maximum where the root is above zero
+            // (times 2^100 it is far above every code) and zero where it is zero
+            const float q = r[k][j] * ri, up = r[k][j] * 0x1p100f;
+            r[k][j] = __builtin_amdgcn_fmed3f(q, up, 0x1p-9f);
+        }
+    if (__any(from_zero)) {
+        asm volatile("");
+        // a moment that starts from zero is the one product g (1 - b1), and products of short gradients often land halfway
+        // between two codes only by their own rounding: what was rounded off (found in 64 bits) decides then
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t u = __float_as_uint(m[k][j]);
+                const double rest = __builtin_fma((double)g[k][j], a.omb1_64, -(double)(g[k][j] * a.omb1));
+                if ((h.m[k] >> (8 * j) & 0x7fu) == 0u && m[k][j] != 0.f && (u & 0x7ffffu) == 0 && (rest > 0.0 || rest < 0.0))
+                    m[k][j] = __uint_as_float((rest > 0.0) == (m[k][j] > 0.f) ? u + 1 : u - 1);
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        h.m[k] = to_e4m3(m[k]);
+        h.v[k] = to_e4m3(r[k]);
+    }
+    h.ms = pow2i(me);
+    h.vs = pow2i(re);
 }
 
-// One block of 256 elements between its loads and its stores.  g, p in, p out; m, v as they are held, in and out.
-template <bool SMALL> struct AwHeld;
-template <> struct AwHeld<false> { f32x4 m, v; };
-template <> struct AwHeld<true> { uint32_t m, v; float ms, vs; };
-
 template <bool SMALL>
-__device__ __forceinline__ void aw_load(AwHeld<SMALL>& h, const AwLaunch& a, long sb, int lane) {
+__device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f32x4 (&g)[4], const AwLaunch& a,
+                                        const AwTensor& t) {
+    f32x4 m[4], v[4], r[4];
+    uint32_t zeros = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (SMALL) {
+            m[k] = from_e4m3(h.m[k]);
+            v[k] = from_e4m3(h.v[k]);
+            const uint32_t w = h.m[k] & 0x7f7f7f7fu;    // a byte of zeros: a code that stands for zero
+            zeros |= (w - 0x01010101u) & ~w;
+        } else {
+            m[k] = h.m[k];
+            v[k] = h.v[k];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (SMALL) {
+                m[k][j] *= h.ms;
+                const float root = v[k][j] * h.vs;
+                v[k][j] = root * root;
+            }
+            m[k][j] = m[k][j] + (g[k][j] - m[k][j]) * a.omb1;
+            v[k][j] = v[k][j] * a.b2 + g[k][j] * g[k][j] * a.omb2;
+            // root and reciprocal of the hardware (one unit in the last place each): the step they scale is added to a
+            // parameter that is larger by orders of magnitude
+            r[k][j] = __builtin_amdgcn_sqrtf(v[k][j]);
+            const float u = m[k][j] * __builtin_amdgcn_rcpf(__builtin_fmaf(r[k][j], t.inv_sqrt_bc2, a.eps));
+            p[k][j] = __builtin_fmaf(-t.step_size, u, p[k][j] * a.decay);
+        }
+    }
     if constexpr (SMALL) {
-        h.m = static_cast<const uint32_t*>(a.m)[sb * 64 + lane];
-        h.v = static_cast<const uint32_t*>(a.v)[sb * 64 + lane];
+        aw_encode(h, m, v, r, g, (zeros & 0x80808080u) != 0u, a);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            h.m[k] = m[k];
+            h.v[k] = v[k];
+        }
+    }
+}
+
+// sb: the row's block of moments; at: the lane's first element in it
+template <bool SMALL>
+__device__ __forceinline__ void aw_load(AwHeld<SMALL>& h, const AwLaunch& a, long sb, int at) {
+    const long i = (sb * AW_BLOCK + at) >> 2;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (SMALL) {
+            h.m[k] = static_cast<const uint32_t*>(a.m)[i + 16 * k];
+            h.v[k] = static_cast<const uint32_t*>(a.v)[i + 16 * k];
+        } else {
+            h.m[k] = static_cast<const f32x4*>(a.m)[i + 16 * k];
+            h.v[k] = static_cast<const f32x4*>(a.v)[i + 16 * k];
+        }
+    }
+    if constexpr (SMALL) {
         h.ms = a.ms[sb];
         h.vs = a.vs[sb];
-    } else {
-        h.m = static_cast<const f32x4*>(a.m)[sb * 64 + lane];
-        h.v = static_cast<const f32x4*>(a.v)[sb * 64 + lane];
     }
 }
-
 template <bool SMALL>
-__device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4& p, f32x4 g, const AwLaunch& a, const AwTensor& t) {
-    f32x4 m, v, r;
-    double tie[4];
-    if constexpr (SMALL) {
-        m = from_e4m3(h.m);
-        v = from_e4m3(h.v);
+__device__ __forceinline__ void aw_store(const AwHeld<SMALL>& h, const AwLaunch& a, long sb, int at) {
+    const long i = (sb * AW_BLOCK + at) >> 2;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m[j] *= h.ms;
-            const float root = v[j] * h.vs;
-            v[j] = root * root;
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (SMALL) {
+            static_cast<uint32_t*>(a.m)[i + 16 * k] = h.m[k];
+            static_cast<uint32_t*>(a.v)[i + 16 * k] = h.v[k];
+        } else {
+            static_cast<f32x4*>(a.m)[i + 16 * k] = h.m[k];
+            static_cast<f32x4*>(a.v)[i + 16 * k] = h.v[k];
         }
-    } else {
-        m = h.m;
-        v = h.v;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float d = g[j] - m[j], add = d * a.omb1;
-        if constexpr (SMALL) tie[j] = m[j] == 0.f ? __builtin_fma((double)d, a.omb1_64, -(double)add) : 0.0;
-        m[j] = m[j] + add;
-        v[j] = v[j] * a.b2 + g[j] * g[j] * a.omb2;
-        // root and reciprocal of the hardware (one unit in the last place each): the step they scale is added to a parameter
-        // that is larger by orders of magnitude
-        r[j] = __builtin_amdgcn_sqrtf(v[j]);
-        p[j] = p[j] * a.decay - t.step_size * (m[j] * __builtin_amdgcn_rcpf(r[j] * t.inv_sqrt_bc2 + a.eps));
     }
     if constexpr (SMALL) {
-        float mm = 0.f, vm = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                   // what is not finite does not set the scale of its neighbours
-            const float am = fabsf(m[j]);
-            mm = fmaxf(mm, am < INFINITY ? am : 0.f);
-            vm = fmaxf(vm, v[j] < INFINITY ? v[j] : 0.f);
-        }
-        // the block's largest root is rounded exactly: it decides the power of two
-        const int me = aw_exponent(aw_wave_max(mm)), re = aw_exponent(sqrtf(aw_wave_max(vm)));
-        const float mi = pow2i(-me), ri = pow2i(-re);
-        f32x4 mq, rq;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mq[j] = m[j] * mi;
-            // a moment that starts from zero is one product, and products of short gradients often land halfway between two
-            // codes only by their own rounding: what was rounded off (found in 64 bits) decides then
-            const uint32_t u = __float_as_uint(mq[j]);
-            if ((tie[j] > 0.0 || tie[j] < 0.0) && mq[j] != 0.f && (u & 0x7ffffu) == 0) mq[j] = __uint_as_float((tie[j] > 0.0) == (mq[j] > 0.f) ? u + 1 : u - 1);
-            rq[j] = r[j] * ri;
-            if (v[j] > 0.f) rq[j] = fmaxf(rq[j], 0x1p-9f);
-        }
-        h.m = to_e4m3(mq);
-        h.v = to_e4m3(rq);
-        h.ms = pow2i(me);
-        h.vs = pow2i(re);
-    } else {
-        h.m = m;
-        h.v = v;
-    }
-}
-
-template <bool SMALL>
-__device__ __forceinline__ void aw_store(const AwHeld<SMALL>& h, const AwLaunch& a, long sb, int lane) {
-    if constexpr (SMALL) {
-        static_cast<uint32_t*>(a.m)[sb * 64 + lane] = h.m;
-        static_cast<uint32_t*>(a.v)[sb * 64 + lane] = h.v;
-        if (lane == 0) {
+        if (at == 0) {
             a.ms[sb] = h.ms;
             a.vs[sb] = h.vs;
         }
-    } else {
-        static_cast<f32x4*>(a.m)[sb * 64 + lane] = h.m;
-        static_cast<f32x4*>(a.v)[sb * 64 + lane] = h.v;
     }
 }
 
 template <typename T, bool SMALL>
 __global__ __launch_bounds__(64 * AW_WAVES) void adamw_multi_kernel(AwLaunch a) {
-    const int lane = threadIdx.x & 63;
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * AW_WAVES + (threadIdx.x >> 6));
     if (unit >= a.units) return;
     uint32_t lo = 0, hi = a.count;                      // the tensor of this unit: the last one with unit0 <= unit
@@ -210,49 +275,60 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_multi_kernel(AwLaunch a) 
     }
     const AwTensor& t = a.t[lo];
     const long b0 = (long)(unit - t.unit0) * AW_UNIT, n = t.n;
-    const long sb0 = (long)t.state_block + b0, i0 = b0 * AW_BLOCK + lane * 4;
+    const int row = (threadIdx.x & 63) >> 4, at = (threadIdx.x & 15) * 4;
+    const long b = b0 + row, i = b * AW_BLOCK + at;
+    f32x4 p[4], g[4];
+    AwHeld<SMALL> h;
     if ((b0 + AW_UNIT) * AW_BLOCK <= n) {               // a whole unit: all its loads go out before the first is needed
-        f32x4 p[AW_UNIT], g[AW_UNIT];
-        AwHeld<SMALL> h[AW_UNIT];
 #pragma unroll
-        for (int k = 0; k < AW_UNIT; ++k) {
-            g[k] = AwIo<T>::load(t.g, i0 + k * AW_BLOCK);
-            p[k] = AwIo<T>::load(t.p, i0 + k * AW_BLOCK);
-            aw_load<SMALL>(h[k], a, sb0 + k, lane);
+        for (int k = 0; k < 4; ++k) {
+            g[k] = AwIo<T>::load(t.g, i + 64 * k);
+            p[k] = AwIo<T>::load(t.p, i + 64 * k);
         }
+        aw_load<SMALL>(h, a, t.state_block + b, at);
+        aw_step<SMALL>(h, p, g, a, t);
 #pragma unroll
-        for (int k = 0; k < AW_UNIT; ++k) {
-            aw_step<SMALL>(h[k], p[k], g[k], a, t);
-            AwIo<T>::store(t.p, i0 + k * AW_BLOCK, p[k]);
-            aw_store<SMALL>(h[k], a, sb0 + k, lane);
-        }
+        for (int k = 0; k < 4; ++k) AwIo<T>::store(t.p, i + 64 * k, p[k]);
+        aw_store<SMALL>(h, a, t.state_block + b, at);
         return;
     }
-    for (int k = 0; k < AW_UNIT && (b0 + k) * AW_BLOCK < n; ++k) {
-        const long i = i0 + k * AW_BLOCK, left = n - i;
-        f32x4 p = {0.f, 0.f, 0.f, 0.f}, g = p;          // behind the tensor: nothing, so that the padding stays zero
-        AwHeld<SMALL> h;
-        aw_load<SMALL>(h, a, sb0 + k, lane);
-        if (left >= 4) {
-            p = AwIo<T>::load(t.p, i);
-            g = AwIo<T>::load(t.g, i);
+    // the end of a tensor: nothing is read behind it, and zeros there keep the padding of its last block zero
+    const bool mine = b * AW_BLOCK < n;
+    if (mine) {
+        aw_load<SMALL>(h, a, t.state_block + b, at);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h.m[k] = h.v[k] = {};
+        if constexpr (SMALL) h.ms = h.vs = 1.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const long x = i + 64 * k;
+        p[k] = g[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (x + 4 <= n) {
+            p[k] = AwIo<T>::load(t.p, x);
+            g[k] = AwIo<T>::load(t.g, x);
         } else {
 #pragma unroll
             for (int j = 0; j < 3; ++j)
-                if (j < left) {
-                    p[j] = AwIo<T>::load1(t.p, i + j);
-                    g[j] = AwIo<T>::load1(t.g, i + j);
+                if (x + j < n) {
+                    p[k][j] = AwIo<T>::load1(t.p, x + j);
+                    g[k][j] = AwIo<T>::load1(t.g, x + j);
                 }
         }
-        aw_step<SMALL>(h, p, g, a, t);
-        if (left >= 4) {
-            AwIo<T>::store(t.p, i, p);
+    }
+    aw_step<SMALL>(h, p, g, a, t);
+    if (mine) aw_store<SMALL>(h, a, t.state_block + b, at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const long x = i + 64 * k;
+        if (x + 4 <= n) {
+            AwIo<T>::store(t.p, x, p[k]);
         } else {
 #pragma unroll
             for (int j = 0; j < 3; ++j)
-                if (j < left) AwIo<T>::store1(t.p, i + j, p[j]);
+                if (x + j < n) AwIo<T>::store1(t.p, x + j, p[k][j]);
         }
-        aw_store<SMALL>(h, a, sb0 + k, lane);
     }
 }
 

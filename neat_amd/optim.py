@@ -11,7 +11,8 @@ parameter groups, gradients that come and go -- with moments in 32 or in 8 bits 
 """
 from __future__ import annotations
 
-import ctypes
+import array
+import operator
 
 import torch
 
@@ -66,6 +67,9 @@ class AdamW(torch.optim.Optimizer):
     def zero_grad(self, set_to_none: bool = False):
         # gradients are views of flat_grad and must stay attached; the backward overwrites them
         self.flat_grad.zero_()
+
+
+_grad_of = operator.attrgetter("grad")
 
 
 class MultiTensorAdamW(torch.optim.Optimizer):
@@ -125,8 +129,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _layout(self, ps):
         """(sizes, the same as a C array, first blocks of the moments as a C array)."""
         sizes = [self._numel[p] for p in ps]
-        longs = ctypes.c_int64 * len(ps)
-        return sizes, longs(*sizes), longs(*[self._first[p] for p in ps])
+        return sizes, array.array("q", sizes), array.array("q", [self._first[p] for p in ps])
 
     @staticmethod
     def _check_group(g):
@@ -148,9 +151,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for i, ps, layout, steps in self._lists:
-            grads = [p.grad for p in ps]
+            grads = list(map(_grad_of, ps))
             at = None
-            if any([g is None for g in grads]):
+            if type(None) in set(map(type, grads)):
                 at = [k for k, g in enumerate(grads) if g is not None]
                 if not at:
                     continue
