@@ -40,6 +40,9 @@ enum {
     NEAT_EPI_F32 = 5             /* out0(f32)  = acc                      (patch embedding)             */
 };
 
+/* element types of entry points that take several */
+enum { NEAT_F32 = 0, NEAT_BF16 = 1 };
+
 const char* neat_version(void);
 const char* neat_last_error(void);
 
@@ -255,7 +258,6 @@ int neat_adamw_flat(float* p, const float* g, float* m, float* v, long n, double
  * each; moment 1 = code * m_scale, SQUARE ROOT of moment 2 = code * v_scale.  The step uses the moments before they are rounded.
  * A value that is not finite becomes a NaN code of its own and leaves its block's scale alone.  Tensors and blocks of one
  * call must not overlap.  The step counts are host values: a captured launch replays them as they were. */
-enum { NEAT_F32 = 0, NEAT_BF16 = 1 };   /* element types */
 int neat_adamw_multi(int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* state_block,
                      const int32_t* step, int dtype, void* m, void* v, float* m_scale, float* v_scale, int state_bits,
                      double lr, double beta1, double beta2, double eps, double wd, void* stream);
@@ -328,6 +330,31 @@ int neat_comm_rank(void);
 int neat_comm_allgather(const void* send, void* recv, long bytes, void* stream);
 int neat_comm_allreduce_f32(const float* send, float* recv, long n, void* stream);
 int neat_comm_destroy(void);
+
+/* ---- log probabilities of given tokens, with entropy, alternatives and gradient (the entropy and contrastive terms of
+ * train_TTA.py:45-48 and zero-shot scoring of evaluation/mcq.py:92-97, for logits that are at hand) ---- */
+/* logits [R, V] of `dtype` (NEAT_F32 / NEAT_BF16), row pitch ld >= V elements, rows aligned to their elements only; z = scale *
+ * logits, scale > 0.  Per row: logp[r] = log softmax(z)[target[r]] (target i64 [R]; negative: 0, there is no target; V or
+ * more: NaN); entropy[r] = -sum p log p; stats f32 [3, R] = (max of the logits, sum exp(z - max z), entropy) for the backward
+ * pass; top_logp f32 [R, k], top_idx i32 [R, k] = the k most probable, best first, ties -> lowest index, k <= 32 and <= V.
+ * logp, entropy, stats may be NULL; target may be NULL with logp.  -inf logits are masked: a row of nothing else has logp =
+ * -inf, entropy 0, alternatives of -inf, gradient 0.  A NaN or +inf makes the row's numbers NaN; a NaN is never an
+ * alternative.  ws: neat_token_logprobs_ws_bytes bytes of device memory, 16-B aligned (0: may be NULL).  V <= 2 097 152 (f32) /
+ * 4 194 304 (bf16; alternatives: V up to 64 pieces of 57 344). */
+long neat_token_logprobs_ws_bytes(int dtype, int R, int V, int k);
+int neat_token_logprobs(const void* logits, long ld, int dtype, const int64_t* target, float scale, int k, float* logp,
+                        float* entropy, float* stats, float* top_logp, int32_t* top_idx, int R, int V, void* ws,
+                        void* stream);
+/* dlogits[r, j] = d(sum_r dlogp[r] logp[r] + dentropy[r] entropy[r]) / dlogits[r, j], of the logits' type, row pitch ld_out;
+ * dlogp, dentropy f32 [R], NULL: zeros.  stats from the forward pass.  dlogits may be logits (same pitch). */
+int neat_token_logprobs_bwd(const void* logits, long ld, int dtype, const int64_t* target, const float* stats,
+                            const float* dlogp, const float* dentropy, float scale, void* dlogits, long ld_out, int R, int V,
+                            void* stream);
+/* Both, for weights that are known beforehand: one reading of rows that fit a workgroup's registers (V <= 32 768 f32, 65 536
+ * bf16), else the two calls above (stats is then required; ws as for k = 0). */
+int neat_token_logprobs_fwd_bwd(const void* logits, long ld, int dtype, const int64_t* target, const float* dlogp,
+                                const float* dentropy, float scale, float* logp, float* entropy, float* stats, void* dlogits,
+                                long ld_out, int R, int V, void* ws, void* stream);
 
 /* f32 -> bf16 cast (weights at load time, n elements) */
 int neat_cast_bf16(const float* src, uint16_t* dst, long n, void* stream);

@@ -76,6 +76,10 @@ SIGNATURES = {
     "neat_comm_allgather": (_I, [_P, _P, _L, _P]),
     "neat_comm_allreduce_f32": (_I, [_P, _P, _L, _P]),
     "neat_comm_destroy": (_I, []),
+    "neat_token_logprobs_ws_bytes": (_L, [_I, _I, _I, _I]),
+    "neat_token_logprobs": (_I, [_P, _L, _I, _P, _F, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P]),
+    "neat_token_logprobs_bwd": (_I, [_P, _L, _I, _P, _P, _P, _P, _F, _P, _L, _I, _I, _P]),
+    "neat_token_logprobs_fwd_bwd": (_I, [_P, _L, _I, _P, _P, _P, _F, _P, _P, _P, _P, _L, _I, _I, _P, _P]),
     "neat_cast_bf16": (_I, [_P, _P, _L, _P]),
     "neat_transpose_cast_bf16": (_I, [_P, _P, _I, _I, _P]),
 }

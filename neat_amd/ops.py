@@ -724,6 +724,104 @@ def mcq_scores(image_features, text_features):
     return logits, pred
 
 
+# ---- log probabilities of given tokens ----
+def _logits2d(t, name):
+    if t.dim() != 2 or t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name}: expected float32 or bfloat16 [rows, vocabulary], got {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a GPU tensor (libneat_hip has no CPU path)")
+    R, V = t.shape
+    if V < 1:
+        raise RuntimeError(f"{name}: an empty vocabulary")
+    ld = t.stride(0) if R > 1 else max(V, t.stride(0))
+    if (V > 1 and t.stride(1) != 1) or ld < V:
+        raise RuntimeError(f"{name}: elements of a row must be adjacent and rows must not overlap (strides {t.stride()})")
+    return R, V, ld
+
+
+def _per_row(t, R, dtype, device, name):
+    if t is None:
+        return None
+    if tuple(t.shape) != (R,) or t.device != device:
+        raise RuntimeError(f"{name}: expected {dtype} [{R}] on the logits' device, got {tuple(t.shape)} on {t.device}")
+    return _p(t, dtype, name)
+
+
+def _lp_ws(dtype, R, V, k, device):
+    n = lib.load().neat_token_logprobs_ws_bytes(_DTYPES[dtype], R, V, k)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _lp_out(out, logits):
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise RuntimeError("token_logprobs: out must have the logits' shape, type and device")
+    if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
+        raise RuntimeError("token_logprobs: out may be the logits themselves, not another view of them")
+    return out, _logits2d(out, "out")[2]
+
+
+def token_logprobs(logits, targets=None, scale=1.0, k=0):
+    """Rows of ``scale * logits`` (float32 or bfloat16 [R, V], any row pitch) -> (logp, entropy, stats, top_logp, top_idx):
+    log probability of ``targets`` (int64 [R]; negative: no target, 0; V or more: NaN; None: logp is None), entropy in nats,
+    the numbers the backward pass needs, and the ``k`` <= 32 most probable entries, best first, ties to the lowest index (None
+    without k).  -inf entries are masked; a row of nothing else has logp and alternatives of -inf and entropy 0."""
+    R, V, ld = _logits2d(logits, "logits")
+    dev, k = logits.device, int(k)
+    if k < 0 or k > 32 or k > V:
+        raise RuntimeError(f"token_logprobs: k={k} must lie in 0 .. min(32, V={V})")
+    tgt = _per_row(targets, R, i64, dev, "targets")
+    logp = torch.empty(R, dtype=f32, device=dev) if targets is not None else None
+    ent = torch.empty(R, dtype=f32, device=dev)
+    stats = torch.empty(3, R, dtype=f32, device=dev)
+    top = torch.empty(R, k, dtype=f32, device=dev) if k else None
+    idx = torch.empty(R, k, dtype=i32, device=dev) if k else None
+    ws = _lp_ws(logits.dtype, R, V, k, dev)
+    with _OnDevice(dev):
+        lib.call("neat_token_logprobs", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, float(scale), k, _p(logp), _p(ent),
+                 _p(stats), _p(top), _p(idx), R, V, _p(ws), _stream())
+    return logp, ent, stats, top, idx
+
+
+def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=1.0, out=None):
+    """Gradient of sum(dlogp * logp + dentropy * entropy) with respect to ``logits``, in their type (``out``: where to write
+    it, the logits themselves allowed).  ``stats`` and ``scale`` are the forward pass's; dlogp / dentropy float32 [R] or None."""
+    R, V, ld = _logits2d(logits, "logits")
+    dev = logits.device
+    if tuple(stats.shape) != (3, R) or stats.device != dev:
+        raise RuntimeError(f"token_logprobs_bwd: stats must be the forward pass's float32 [3, {R}]")
+    if dlogp is not None and targets is None:
+        raise RuntimeError("token_logprobs_bwd: dlogp needs targets")
+    tgt, a, b = (_per_row(t, R, d, dev, n) for t, d, n in ((targets, i64, "targets"), (dlogp, f32, "dlogp"),
+                                                           (dentropy, f32, "dentropy")))
+    out, ldo = _lp_out(out, logits)
+    with _OnDevice(dev):
+        lib.call("neat_token_logprobs_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, _p(stats, f32, "stats"), a, b,
+                 float(scale), out.data_ptr(), ldo, R, V, _stream())
+    return out
+
+
+def token_logprobs_fwd_bwd(logits, targets, dlogp=None, dentropy=None, scale=1.0, out=None):
+    """(logp, entropy, dlogits) of ``token_logprobs`` and ``token_logprobs_bwd`` for weights that are known beforehand (a mean
+    over rows, a mask): one reading of the logits where a row fits a workgroup's registers."""
+    R, V, ld = _logits2d(logits, "logits")
+    dev = logits.device
+    if dlogp is not None and targets is None:
+        raise RuntimeError("token_logprobs_fwd_bwd: dlogp needs targets")
+    tgt, a, b = (_per_row(t, R, d, dev, n) for t, d, n in ((targets, i64, "targets"), (dlogp, f32, "dlogp"),
+                                                           (dentropy, f32, "dentropy")))
+    logp = torch.empty(R, dtype=f32, device=dev) if targets is not None else None
+    ent = torch.empty(R, dtype=f32, device=dev)
+    out, ldo = _lp_out(out, logits)
+    ws = _lp_ws(logits.dtype, R, V, 0, dev)
+    stats = torch.empty(3, R, dtype=f32, device=dev) if ws is not None else None
+    with _OnDevice(dev):
+        lib.call("neat_token_logprobs_fwd_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, a, b, float(scale),
+                 _p(logp), _p(ent), _p(stats), out.data_ptr(), ldo, R, V, _p(ws), _stream())
+    return logp, ent, out
+
+
 def gemm_f32_nt(A, B):
     M, K = A.shape
     N = B.shape[0]

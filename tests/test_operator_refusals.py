@@ -60,3 +60,40 @@ def test_adamw_multi_wrapper_refuses():
         MultiTensorAdamW([torch.nn.Parameter(p)], betas=(0.9, 1.0))
     with pytest.raises(ValueError):
         MultiTensorAdamW([torch.nn.Parameter(p)], lr=-1.0)
+
+
+def _lp(z=64, ld=100, dtype=0, target=64, scale=1.0, k=0, logp=64, top=64, idx=64, R=4, V=100, ws=64):
+    return lib.load().neat_token_logprobs(z, ld, dtype, target, scale, k, logp, 64, 64, top, idx, R, V, ws, None)
+
+
+@pytest.mark.parametrize("bad, rc, says", [
+    (dict(z=None), -2, "null"), (dict(target=None), -2, "targets"), (dict(dtype=2), -2, "dtype"), (dict(ld=99), -1, "pitch"),
+    (dict(V=0), -1, "V=0"), (dict(R=-1), -1, "R=-1"), (dict(k=33), -1, "k=33"), (dict(k=5, V=4), -1, "k=5"),
+    (dict(k=-1), -1, "k=-1"), (dict(k=2, top=None), -2, "alternatives"), (dict(z=66), -2, "aligned"),
+    (dict(scale=0.0), -2, "scale"), (dict(scale=-1.0), -2, "scale"), (dict(scale=float("nan")), -2, "scale"),
+    (dict(scale=float("inf")), -2, "scale"), (dict(V=3_000_000, ld=3_000_000), -1, "above"),
+    (dict(V=100_000, ld=100_000, ws=None), -2, "workspace"), (dict(V=4_100_000, ld=4_100_000, dtype=1, k=32), -1, "pieces")])
+def test_token_logprobs_checks_before_launching(bad, rc, says):
+    assert _lp(**bad) == rc
+    assert says in lib.last_error()
+
+
+def test_token_logprobs_gradient_checks_before_launching():
+    L = lib.load()
+    assert L.neat_token_logprobs_bwd(64, 9, 0, 64, None, 64, 64, 1.0, 64, 9, 2, 9, None) == -2
+    assert L.neat_token_logprobs_bwd(64, 9, 0, None, 64, 64, 64, 1.0, 64, 9, 2, 9, None) == -2
+    assert L.neat_token_logprobs_bwd(64, 9, 0, 64, 64, 64, 64, 1.0, 64, 8, 2, 9, None) == -1
+    assert L.neat_token_logprobs_bwd(64, 9, 0, 64, 64, 64, 64, 1.0, 65, 9, 2, 9, None) == -2
+    assert L.neat_token_logprobs_fwd_bwd(64, 9, 0, None, 64, 64, 1.0, 64, 64, 64, 64, 9, 2, 9, None, None) == -2
+    assert L.neat_token_logprobs_fwd_bwd(64, 90000, 0, 64, 64, 64, 1.0, 64, 64, None, 64, 90000, 2, 90000, 64, None) == -2
+    assert L.neat_token_logprobs_ws_bytes(0, 4, 32768, 0) == 0
+    assert L.neat_token_logprobs_ws_bytes(0, 4, 32769, 0) >= 4 * 2 * 16
+    assert _lp(R=0) == 0
+
+
+def test_token_logprobs_wrapper_refuses():
+    z = torch.zeros(3, 7)
+    for call in (lambda: ops.token_logprobs(z), lambda: ops.token_logprobs(z.half()), lambda: ops.token_logprobs(z[0]),
+                 lambda: ops.token_logprobs_bwd(z, None, torch.zeros(3, 3)), lambda: ops.token_logprobs_fwd_bwd(z, None)):
+        with pytest.raises(RuntimeError):
+            call()
