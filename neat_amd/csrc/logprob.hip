@@ -10,9 +10,10 @@
 // What a mask leaves out is -inf: probability 0, no share in H, gradient 0.  A row with nothing left has logp = -inf, H = 0,
 // alternatives of -inf and no gradient.  NaN (or +inf) makes the row's results NaN; it is never an alternative itself.
 //
-// Alternatives: every element is a 64-bit key (ordered value, then lower index first), so keys never tie.  The k-th largest of
-// up to 256 group maxima bounds the k-th largest key from below, at most k groups hold candidates above it, and those are
-// ranked by counting: no sort, no atomics that matter to the result, and the same work for a row of equal values.
+// Alternatives: the k-th largest of 64 group maxima bounds the k-th largest value from below; the few values that reach it are
+// collected and ranked by counting (value, then lower index): no sort, and no atomic that matters to the result.  Where many
+// reach it (a row of few different values, or mostly masked), 64-bit keys (value, index) that never tie take its place: the
+// k-th largest of up to 256 groups' keys leaves at most k groups' elements, for which there is room.
 #include "wave.h"
 
 namespace neat {
@@ -159,10 +160,114 @@ __device__ __forceinline__ u32x4 lp_grad_vec(u32x4 raw, const LpGrad& q, float c
 
 enum { LP_SUMS = 0, LP_TOP = 1, LP_GRAD = 2 };
 
-// One workgroup, one row (or one piece of it).
+constexpr int LP_FEW = 256;                  // candidates of the first bound that are ranked; more go by keys
+
+// the k largest of the `total` keys in `cand`, in order
+template <int THREADS>
+__device__ __forceinline__ void lp_rank(const LpArgs& g, const uint64_t* cand, int total, int row, int piece, const LpRow& r,
+                                        float s) {
+    const int k = g.k;
+    for (int i = threadIdx.x; i < total; i += THREADS) {
+        const uint64_t own = cand[i];
+        int rank = 0;
+        for (int q = 0; q < total; ++q) rank += cand[q] > own ? 1 : 0;
+        if (rank < k) {
+            if (g.part) {
+                g.keys[((long)row * g.S + piece) * k + rank] = own;
+            } else {
+                g.idx[(long)row * k + rank] = lp_index(own);
+                g.top[(long)row * k + rank] = lp_logp(lp_value(own), r, s, g.scale);
+            }
+        }
+    }
+    if (g.part)
+        for (int i = total + threadIdx.x; i < k; i += THREADS) g.keys[((long)row * g.S + piece) * k + i] = 0;
+}
+
+// raw: this lane's elements; lane_m: the largest of them; least: a bound that at least k elements reach; *count is 0
+template <typename T, int THREADS>
+__device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, const u32x4 (&raw)[LP_NV], int row, int piece, int lo,
+                                                int n, float lane_m, float least, int* count, const LpRow& r, float s) {
+    constexpr int VEC = LpIo<T>::VEC, GROUPS = THREADS < 256 ? THREADS : 256, GL = THREADS / GROUPS;
+    extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
+    const int tid = threadIdx.x;
+    // NaN counts as -inf, which is why the comparisons are turned round
+    if (!(lane_m < least)) {
+#pragma unroll
+        for (int i = 0; i < LP_NV; ++i) {
+            const int e = (tid + i * THREADS) * VEC;
+            uint32_t hit = 0;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) hit |= !(LpIo<T>::get(raw[i], j) < least) ? 1u << j : 0u;
+            if (e < n) {
+                for (; hit; hit &= hit - 1) {
+                    const int x = e + __builtin_ctz(hit);
+                    if (x < n) {
+                        const int at = atomicAdd(count, 1);
+                        if (at < LP_FEW) cand[at] = lp_key(LpIo<T>::one(z, x), lo + x);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int total = *count;
+    if (total <= LP_FEW) {
+        lp_rank<THREADS>(g, cand, total, row, piece, r, s);
+        return;
+    }
+    // many values reach the bound: the same once more with keys that never tie, from memory (the row is in the caches)
+    __shared__ uint64_t group[GROUPS];
+    __shared__ uint64_t bound;
+    __syncthreads();
+    uint64_t mine = 0;
+    for (int first = tid * VEC; first < n; first += THREADS * VEC) {
+        const int last = min(first + VEC, n);
+        for (int e = first; e < last; ++e) {
+            const uint64_t key = lp_key(LpIo<T>::one(z, e), lo + e);
+            mine = key > mine ? key : mine;
+        }
+    }
+    uint64_t best = mine;
+#pragma unroll
+    for (int o = 1; o < GL; o <<= 1) {
+        const uint64_t other = lp_shfl_xor(best, o);
+        best = other > best ? other : best;
+    }
+    if (tid % GL == 0) group[tid / GL] = best;
+    if (tid == 0) {
+        bound = 0;
+        *count = 0;
+    }
+    __syncthreads();
+    {                                        // the k-th largest group: the GL lanes of a group count its betters together
+        const uint64_t own = group[tid / GL];
+        int rank = 0;
+        for (int q = tid % GL; q < GROUPS; q += GL) rank += group[q] > own ? 1 : 0;
+#pragma unroll
+        for (int o = 1; o < GL; o <<= 1) rank += __shfl_xor(rank, o);
+        if (rank == g.k - 1 && own != 0 && tid % GL == 0) bound = own;       // fewer groups than k: everything is a candidate
+    }
+    __syncthreads();
+    const uint64_t floor_key = bound;
+    if (mine != 0 && mine >= floor_key) {
+        for (int first = tid * VEC; first < n; first += THREADS * VEC) {
+            const int last = min(first + VEC, n);
+            for (int e = first; e < last; ++e) {
+                const uint64_t key = lp_key(LpIo<T>::one(z, e), lo + e);
+                if (key >= floor_key) cand[atomicAdd(count, 1)] = key;
+            }
+        }
+    }
+    __syncthreads();
+    lp_rank<THREADS>(g, cand, *count, row, piece, r, s);
+}
+
+// One workgroup, one row (or one piece of it).  1 024 lanes: at most 64 registers, so that two rows share a CU and one loads
+// while the other computes.
 template <typename T, int THREADS, int MODE>
-__global__ __launch_bounds__(THREADS) void logprob_kernel(LpArgs g) {
-    constexpr int VEC = LpIo<T>::VEC, WAVES = THREADS / 64, GROUPS = THREADS < 256 ? THREADS : 256, GL = THREADS / GROUPS;
+__global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kernel(LpArgs g) {
+    constexpr int VEC = LpIo<T>::VEC, WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = g.row0 + blockIdx.x / g.S, piece = blockIdx.x % g.S;
     const int lo = piece * g.chunk, n = min(g.chunk, g.V - lo);
@@ -182,27 +287,16 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LpArgs g) {
                 if (e + j < n) LpIo<T>::put(raw[i], j, LpIo<T>::one(z, e + j));
         }
     }
-    float m = -INFINITY;
-    int mi = tid * VEC;                      // index of the lane's largest element (its first one where all are masked)
+    float lane_m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < LP_NV; ++i) {
         if (i * THREADS * VEC < n) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float x = LpIo<T>::get(raw[i], j);
-                if constexpr (MODE == LP_TOP) {
-                    if (x > m) {
-                        m = x;
-                        mi = (tid + i * THREADS) * VEC + j;
-                    }
-                } else {
-                    m = fmaxf(m, x);
-                }
-            }
+            for (int j = 0; j < VEC; ++j) lane_m = fmaxf(lane_m, LpIo<T>::get(raw[i], j));
         }
     }
-    const float lane_m = m;
-    m = wave_max_f(m);
+    const float row_m = row_max(lane_m);     // of 16 lanes
+    const float m = fmaxf(fmaxf(lane_f(row_m, 0), lane_f(row_m, 16)), fmaxf(lane_f(row_m, 32), lane_f(row_m, 48)));
     const float m0 = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
 #pragma unroll
@@ -218,40 +312,56 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LpArgs g) {
     }
     LpSums v{m, wave_sum_f(s), wave_sum_f(t)};
 
-    __shared__ float red[3][16];
-    __shared__ uint64_t group[GROUPS];
-    __shared__ uint64_t bound;
+    // what the first wave finds out for all: the row's sums, and the least value of a candidate
+    __shared__ float red[3][WAVES], group[64], joined[4];
     __shared__ int count;
-    extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
-    uint64_t mine = 0;
-    if constexpr (MODE == LP_TOP) {
-        mine = mi < n ? lp_key(lane_m, lo + mi) : 0;
-        uint64_t best = mine;
-#pragma unroll
-        for (int o = 1; o < GL; o <<= 1) {
-            const uint64_t other = lp_shfl_xor(best, o);
-            best = other > best ? other : best;
-        }
-        if (tid % GL == 0) group[tid / GL] = best;
-        if (tid == 0) {
-            bound = 0;
-            count = 0;
-        }
+    constexpr int GL = THREADS / 64;         // lanes of the 64 groups: one, a quad or a row of 16
+    float group_m = lane_m;
+    if constexpr (GL >= 4) {
+        group_m = fmaxf(group_m, dpp_f<DPP_XOR1>(group_m));
+        group_m = fmaxf(group_m, dpp_f<DPP_XOR2>(group_m));
     }
-    if (WAVES > 1) {
+    if constexpr (GL == 16) group_m = row_m;
+    if constexpr (WAVES > 1) {
         if (lane == 0) {
             red[0][wave] = v.m;
             red[1][wave] = v.s;
             red[2][wave] = v.t;
         }
-        __syncthreads();
-        v = LpSums{-INFINITY, 0.f, 0.f};
-        if (lane < WAVES) v = LpSums{red[0][lane], red[1][lane], red[2][lane]};
-        v = lp_join(v, c);
-    } else if (MODE == LP_TOP) {
+        if (MODE == LP_TOP && tid % GL == 0) group[tid / GL] = group_m;
         __syncthreads();
     }
-
+    if (wave == 0) {
+        if constexpr (WAVES > 1) {
+            v = LpSums{-INFINITY, 0.f, 0.f};
+            if (lane < WAVES) v = LpSums{red[0][lane], red[1][lane], red[2][lane]};
+            v = lp_join(v, c);
+        }
+        float least = 0.f;
+        if constexpr (MODE == LP_TOP) {      // k-th largest of 64: every lane counts what is above and what is not below its own
+            const float own = WAVES > 1 ? group[lane] : group_m;
+            int above = 0, reach = 0;
+#pragma unroll 8
+            for (int q = 0; q < 64; ++q) {
+                const float other = lane_f(own, q);
+                above += other > own ? 1 : 0;
+                reach += other >= own ? 1 : 0;
+            }
+            const uint64_t hit = __ballot(above < g.k && reach >= g.k);
+            least = lane_f(own, __builtin_ctzll(hit));
+            if (lane == 0) count = 0;
+        }
+        if (lane == 0) {
+            joined[0] = v.m;
+            joined[1] = v.s;
+            joined[2] = v.t;
+            joined[3] = least;
+        }
+    }
+    if constexpr (WAVES > 1 || MODE == LP_TOP) {
+        __syncthreads();
+        v = LpSums{joined[0], joined[1], joined[2]};
+    }
     const LpRow r = lp_row(v);
     if (tid == 0) {
         if (g.part) {
@@ -263,47 +373,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LpArgs g) {
             lp_write_row<T>(g, row, v, r);
         }
     }
-    if constexpr (MODE == LP_TOP) {
-        const int k = g.k;
-        {                                    // the k-th largest group: the GL lanes of a group count its betters together
-            const uint64_t own = group[tid / GL];
-            int rank = 0;
-            for (int q = tid % GL; q < GROUPS; q += GL) rank += group[q] > own ? 1 : 0;
-#pragma unroll
-            for (int o = 1; o < GL; o <<= 1) rank += __shfl_xor(rank, o);
-            if (rank == k - 1 && own != 0 && tid % GL == 0) bound = own;     // fewer groups than k: everything is a candidate
-        }
-        __syncthreads();
-        const uint64_t least = bound;
-        if (mine != 0 && mine >= least) {
-#pragma unroll
-            for (int i = 0; i < LP_NV; ++i) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int e = (tid + i * THREADS) * VEC + j;
-                    const uint64_t key = lp_key(LpIo<T>::get(raw[i], j), lo + e);
-                    if (e < n && key >= least) cand[atomicAdd(&count, 1)] = key;
-                }
-            }
-        }
-        __syncthreads();
-        const int total = count;
-        for (int i = tid; i < total; i += THREADS) {
-            const uint64_t own = cand[i];
-            int rank = 0;
-            for (int q = 0; q < total; ++q) rank += cand[q] > own ? 1 : 0;
-            if (rank < k) {
-                if (g.part) {
-                    g.keys[((long)row * g.S + piece) * k + rank] = own;
-                } else {
-                    g.idx[(long)row * k + rank] = lp_index(own);
-                    g.top[(long)row * k + rank] = lp_logp(lp_value(own), r, v.s, g.scale);
-                }
-            }
-        }
-        if (g.part)
-            for (int i = total + tid; i < k; i += THREADS) g.keys[((long)row * g.S + piece) * k + i] = 0;
-    }
+    if constexpr (MODE == LP_TOP) lp_alternatives<T, THREADS>(g, z, raw, row, piece, lo, n, lane_m, joined[3], &count, r, v.s);
     if constexpr (MODE == LP_GRAD) {
         const LpGrad q = lp_grad(g, row, r.m0, v.s, r.ent);
         T* dz = static_cast<T*>(g.dz) + (long)row * g.ldz;
@@ -417,7 +487,8 @@ static LpPlan lp_plan(int vec, int V, int k) {
 }
 static size_t lp_cand_bytes(const LpPlan& p, int vec, int k) {
     const int gl = p.threads <= 256 ? 1 : 4;
-    return (size_t)k * gl * cdiv(p.chunk, (long)p.threads * vec) * vec * 8;
+    const size_t b = (size_t)k * gl * cdiv(p.chunk, (long)p.threads * vec) * vec * 8;
+    return b > LP_FEW * 8 ? b : LP_FEW * 8;
 }
 static long lp_part_bytes(long R, const LpPlan& p) { return p.S == 1 ? 0 : (R * p.S * 16 + 255) / 256 * 256; }
 
