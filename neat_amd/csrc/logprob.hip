@@ -395,36 +395,60 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
     }
 }
 
-// Joins the pieces of a row: one wave, one row.
-template <typename T>
-__global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs g) {
-    const int row = g.row0 + blockIdx.x, lane = threadIdx.x;
+// Joins the pieces of a row: one workgroup, one row.  The lists are in order, so the k-th largest of all is at least every
+// list's k-th and, S ceil(k / S) keys being at least k, the least of the lists' ceil(k / S)-th: only keys that reach both are
+// ranked (one of them after the other, a wave's maximum each, took 0.4 us a key).
+constexpr int LPJ_THREADS = 256;
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void logprob_join_kernel(LpArgs g) {
+    __shared__ float joined[3];
+    __shared__ uint64_t bound;
+    __shared__ int count;
+    extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
+    const int row = g.row0 + blockIdx.x, lane = threadIdx.x & 63;
     const float c = g.scale * LOG2E;
-    LpSums v{-INFINITY, 0.f, 0.f};
-    if (lane < g.S) {
-        const float* p = g.part + ((long)row * g.S + lane) * 4;
-        v = LpSums{p[0], p[1], p[2]};
-    }
-    v = lp_join(v, c);
-    const LpRow r = lp_row(v);
-    if (lane == 0) lp_write_row<T>(g, row, v, r);
-    if (g.k == 0) return;
-    const uint64_t* list = g.keys + ((long)row * g.S + lane) * g.k;      // this lane's list, best first
-    int next = 0;
-    uint64_t head = lane < g.S ? list[0] : 0;
-    for (int i = 0; i < g.k; ++i) {
-        uint64_t best = head;
+    const uint64_t* keys = g.keys + (long)row * g.S * g.k;
+    if (threadIdx.x < 64) {
+        LpSums v{-INFINITY, 0.f, 0.f};
+        if (lane < g.S) {
+            const float* p = g.part + ((long)row * g.S + lane) * 4;
+            v = LpSums{p[0], p[1], p[2]};
+        }
+        v = lp_join(v, c);
+        if (lane == 0) lp_write_row<T>(g, row, v, lp_row(v));
+        if (THREADS > 64) {
+            uint64_t last = 0, early = ~0ull;
+            if (lane < g.S) {
+                last = keys[(long)lane * g.k + g.k - 1];
+                early = keys[(long)lane * g.k + (g.k + g.S - 1) / g.S - 1];
+            }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = lp_shfl_xor(best, o);
-            best = other > best ? other : best;
-        }
-        if (head == best && best != 0) head = ++next < g.k ? list[next] : 0;
-        if (lane == 0) {
-            g.idx[(long)row * g.k + i] = lp_index(best);
-            g.top[(long)row * g.k + i] = lp_logp(lp_value(best), r, v.s, g.scale);
+            for (int o = 32; o > 0; o >>= 1) {
+                const uint64_t a = lp_shfl_xor(last, o), b = lp_shfl_xor(early, o);
+                last = a > last ? a : last;
+                early = b < early ? b : early;
+            }
+            if (lane == 0) {
+                joined[0] = v.m;
+                joined[1] = v.s;
+                joined[2] = v.t;
+                bound = last > early ? last : early;
+                count = 0;
+            }
         }
     }
+    if (THREADS == 64) return;
+    __syncthreads();
+    const uint64_t least = bound > 0 ? bound : 1;               // 0: a list shorter than k has no key there
+    for (int i = threadIdx.x; i < g.S * g.k; i += THREADS) {
+        const uint64_t key = keys[i];
+        if (key >= least) cand[atomicAdd(&count, 1)] = key;
+    }
+    __syncthreads();
+    const LpSums v{joined[0], joined[1], joined[2]};
+    const LpRow r = lp_row(v);
+    g.part = nullptr;                                           // ranked into the results
+    lp_rank<THREADS>(g, cand, count, row, 0, r, v.s);
 }
 
 // The gradient from a forward pass's numbers: every lane reads and writes its own elements, so that dz may be the logits.
@@ -517,7 +541,10 @@ static int lp_forward(LpArgs& g, const LpPlan& p, hipStream_t s) {
     int rc = g.k > 0 ? lp_launch<T, LP_TOP>(g, p, lp_cand_bytes(p, LpIo<T>::VEC, g.k), what, s)
                      : lp_launch<T, LP_SUMS>(g, p, 0, what, s);
     if (rc || g.S == 1) return rc;
-    return lp_rows(g, 1, 64, what, [&](dim3 grid) { hipLaunchKernelGGL(logprob_join_kernel<T>, grid, dim3(64), 0, s, g); });
+    return lp_rows(g, 1, LPJ_THREADS, what, [&](dim3 grid) {
+        if (g.k == 0) hipLaunchKernelGGL((logprob_join_kernel<T, 64>), grid, dim3(64), 0, s, g);
+        else hipLaunchKernelGGL((logprob_join_kernel<T, LPJ_THREADS>), grid, dim3(LPJ_THREADS), (size_t)g.S * g.k * 8, s, g);
+    });
 }
 template <typename T>
 static int lp_backward(LpArgs g, hipStream_t s) {

@@ -7,6 +7,7 @@ raise RuntimeError on any failure -- there is no eager fallback.
 from __future__ import annotations
 
 import array
+import functools
 import operator
 import os
 from typing import Optional, Tuple
@@ -520,19 +521,14 @@ def adamw_flat(p, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0):
              float(beta1), float(beta2), float(eps), float(wd), int(step), _stream())
 
 
-class _OnDevice:
-    """Makes the tensors' device current for a launch where it is not (the library launches on the current device)."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == _device_index() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call_on(device, name, *args):
+    """lib.call with the current stream of ``device``, which is made current where it is not (the library launches on the
+    current device)."""
+    if device.index == _device_index():
+        lib.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            lib.call(name, *args, _stream())
 
 
 def _device_index() -> int:
@@ -604,10 +600,9 @@ def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, 
                            "capture the backward pass and step outside the graph")
     p_c, g_c = array.array("Q", map(_ptr_of, params)), array.array("Q", map(_ptr_of, grads))
     steps_c = array.array("i", steps)
-    with _OnDevice(first.device):
-        lib.call("neat_adamw_multi", count, p_c.buffer_info()[0], g_c.buffer_info()[0], sizes_c.buffer_info()[0],
-                 blocks_c.buffer_info()[0], steps_c.buffer_info()[0], _DTYPES[dtype], _p(m), _p(v), _p(m_scale, f32, "m_scale"),
-                 _p(v_scale, f32, "v_scale"), 8 if m.dtype == torch.uint8 else 32, lr, beta1, beta2, eps, wd, _stream())
+    _call_on(first.device, "neat_adamw_multi", count, p_c.buffer_info()[0], g_c.buffer_info()[0], sizes_c.buffer_info()[0],
+             blocks_c.buffer_info()[0], steps_c.buffer_info()[0], _DTYPES[dtype], _p(m), _p(v), _p(m_scale, f32, "m_scale"),
+             _p(v_scale, f32, "v_scale"), 8 if m.dtype == torch.uint8 else 32, lr, beta1, beta2, eps, wd)
 
 
 # ---- retrieval ----
@@ -747,9 +742,18 @@ def _per_row(t, R, dtype, device, name):
     return _p(t, dtype, name)
 
 
+@functools.lru_cache(maxsize=256)
+def _lp_ws_bytes(dtype, R, V, k):
+    return lib.load().neat_token_logprobs_ws_bytes(_DTYPES[dtype], R, V, k)
+
+
 def _lp_ws(dtype, R, V, k, device):
-    n = lib.load().neat_token_logprobs_ws_bytes(_DTYPES[dtype], R, V, k)
+    n = _lp_ws_bytes(dtype, R, V, k)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _lp_out(out, logits):
@@ -778,9 +782,8 @@ def token_logprobs(logits, targets=None, scale=1.0, k=0):
     top = torch.empty(R, k, dtype=f32, device=dev) if k else None
     idx = torch.empty(R, k, dtype=i32, device=dev) if k else None
     ws = _lp_ws(logits.dtype, R, V, k, dev)
-    with _OnDevice(dev):
-        lib.call("neat_token_logprobs", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, float(scale), k, _p(logp), _p(ent),
-                 _p(stats), _p(top), _p(idx), R, V, _p(ws), _stream())
+    _call_on(dev, "neat_token_logprobs", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, float(scale), k, _ptr(logp),
+             ent.data_ptr(), stats.data_ptr(), _ptr(top), _ptr(idx), R, V, _ptr(ws))
     return logp, ent, stats, top, idx
 
 
@@ -796,9 +799,8 @@ def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=
     tgt, a, b = (_per_row(t, R, d, dev, n) for t, d, n in ((targets, i64, "targets"), (dlogp, f32, "dlogp"),
                                                            (dentropy, f32, "dentropy")))
     out, ldo = _lp_out(out, logits)
-    with _OnDevice(dev):
-        lib.call("neat_token_logprobs_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, _p(stats, f32, "stats"), a, b,
-                 float(scale), out.data_ptr(), ldo, R, V, _stream())
+    _call_on(dev, "neat_token_logprobs_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, _p(stats, f32, "stats"), a, b,
+             float(scale), out.data_ptr(), ldo, R, V)
     return out
 
 
@@ -816,9 +818,8 @@ def token_logprobs_fwd_bwd(logits, targets, dlogp=None, dentropy=None, scale=1.0
     out, ldo = _lp_out(out, logits)
     ws = _lp_ws(logits.dtype, R, V, 0, dev)
     stats = torch.empty(3, R, dtype=f32, device=dev) if ws is not None else None
-    with _OnDevice(dev):
-        lib.call("neat_token_logprobs_fwd_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, a, b, float(scale),
-                 _p(logp), _p(ent), _p(stats), out.data_ptr(), ldo, R, V, _p(ws), _stream())
+    _call_on(dev, "neat_token_logprobs_fwd_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, a, b, float(scale),
+             _ptr(logp), ent.data_ptr(), _ptr(stats), out.data_ptr(), ldo, R, V, _ptr(ws))
     return logp, ent, out
 
 
