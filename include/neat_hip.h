@@ -68,6 +68,30 @@ int neat_ln_bwd_finalize(const float* partial, int nblk, int cols, float* dgamma
 int neat_ln_bwd_finalize_batched(const float* partial, int nblk, int cols, int count, float* const* dst,
                                  int accumulate, void* stream);
 
+/* ---- the norms around a block with its gate and residual scale (LayerScale, open_clip/transformer.py:46-53, :234-243; norms
+ * behind the branches, :246-289) ---- */
+/* n = N_post(h) (post_w NULL: h); x_out = x + n * scale[c] * gate[g, c]; y = N_pre(x_out).  kind: NEAT_NORM_LAYER (mean taken
+ * off, biased variance) or NEAT_NORM_RMS, both norms alike, eps inside the root.  x, x_out f32 [rows, cols] (x_out may be x);
+ * h, y of `dtype` (NEAT_F32 / NEAT_BF16); weights, scale f32 [cols], gate f32 [groups, cols]; pre_b, post_w, post_b, scale,
+ * gate may be NULL.  Row r belongs to group r / (rows / groups), or with cu (device i32 [groups + 1], ascending from 0, read
+ * within the rows) to the g with cu[g] <= r < cu[g + 1]; rows from cu[groups] on are left as they are, or zeroed in the
+ * first (zero_rest & 1: x_out, dx) and second output (& 2: y, dh).  stats f32 [4, rows] = (mean, 1/deviation) of h and of x_out for the backward pass, or NULL.
+ * cols % 4 == 0, <= 4 096; f32 arrays 16-byte aligned, bf16 ones 8. */
+enum { NEAT_NORM_LAYER = 0, NEAT_NORM_RMS = 1 };
+int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const float* pre_w, const float* pre_b,
+                      const float* post_w, const float* post_b, const float* scale, const float* gate, int groups,
+                      const int32_t* cu, float* x_out, void* y, float* stats, int zero_rest, int rows, int cols, float eps,
+                      void* stream);
+/* dy (of dtype) = gradient of y, dres f32 [rows, cols] = gradient of x_out from elsewhere (NULL: none; may be dx) -> dx f32
+ * (gradient of x) and dh (of dtype), and the sums over rows dpre_w .. dscale f32 [cols], dgate f32 [groups, cols] (NULL: not
+ * wanted; written, not added to).  stats, x_out from the forward pass.  ws: neat_res_norm_ws_floats floats, 16-byte aligned.
+ * Sums are formed in a fixed order. */
+long neat_res_norm_ws_floats(int rows, int cols, int groups);
+int neat_res_norm_bwd(const void* dy, const float* dres, const void* h, const float* x_out, const float* stats, int dtype, int kind,
+                      const float* pre_w, const float* post_w, const float* post_b, const float* scale, const float* gate,
+                      int groups, const int32_t* cu, float* dx, void* dh, float* dpre_w, float* dpre_b, float* dpost_w,
+                      float* dpost_b, float* dscale, float* dgate, float* ws, int zero_rest, int rows, int cols, void* stream);
+
 /* ---- bf16 MFMA GEMM: nn.Linear / MHA projections, open_clip/transformer.py:209-213,227-229 ---- */
 /* Frozen weights are packed ONCE into MFMA-fragment order (bf16).  Logical matrix Wl[N,K]:
  *   transposed == 0: Wl = src, row-major f32 [N,K]           (forward: nn.Linear.weight [out,in])

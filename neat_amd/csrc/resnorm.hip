@@ -1,0 +1,537 @@
+// The norms before and after a block, fused with its gate and residual scale, forward and backward.
+//
+//   n = N_post(h)  (or h);   x' = x + n * scale[c] * gate[g(row), c];   y = N_pre(x')
+//   N(u) = uh * w + b,  uh = (u - mean u) / sqrt(var u + eps)  (LayerNorm)  or  u / sqrt(mean u^2 + eps)  (RMS)
+// h is a block's output (attention, MLP), x the residual stream it joins, y what the next block reads: LayerScale
+// (reference open_clip/transformer.py:46-53, :234-243), norms behind the block (:246-289), gates of conditioned blocks.
+// Backward, e = d/dx':
+//   e = dres + N_pre'(dy);   dx = e;   dn = e * scale * gate;   dh = N_post'(dn)
+//   dw_pre = sum dy xh, db_pre = sum dy, dw_post = sum dn hh, db_post = sum dn, dgate[g] = scale * sum_{rows of g} e n,
+//   dscale = sum_g gate[g] * sum_{rows of g} e n
+//   N'(d) = r (z - mean z - uh mean(z uh)), z = d w (RMS: without mean z)
+//
+// Both directions read every input once and write every output once: 8 + 2t bytes an element forward, 12 + 3t backward (t = 2
+// for bf16, 4 for fp32).  A team of 1, 2 or 4 waves holds a row (up to 1 024 columns a wave, four 16-B chunks a lane) in
+// registers and takes a contiguous run of rows, balanced to one row whatever the groups' lengths.  Column sums stay in
+// registers over the run.  A group's sum is left behind at each group's end in slot team + group: runs and groups advance
+// together, so no two (team, group) pairs share a slot, and a second launch adds each group's slots, and the column sums, in
+// a fixed order: no atomics, equal bits on every run.
+#include "wave.h"
+
+namespace neat {
+
+constexpr int RN_MAX_COLS = 4096;
+constexpr int RN_FWD_WAVES = 4, RN_BWD_WAVES = 8;         // waves of a workgroup whose teams are single waves
+constexpr int RN_SUMS = 5;                                // column sums: pre_w, pre_b, post_w, post_b, scale
+
+struct RnArgs {
+    const float* x;                                       // [rows, cols]; the backward pass's x' stands here
+    const void* h;
+    const float *pre_w, *pre_b, *post_w, *post_b, *scale, *gate;
+    const int32_t* cu;                                    // [groups + 1] or null: groups of rows / groups rows
+    float* x_out;
+    void* y;
+    float* stats;                                         // [4, rows]: mean, 1/deviation of h; of x'
+    const void* dy;
+    const float* dres;
+    float* dx;
+    void* dh;
+    float* part;                                          // [workgroups, RN_SUMS, cols]
+    float* slots;                                         // [teams + groups, cols]
+    int rows, cols, groups, teams;
+    int rms, zero_rest;
+    float eps;
+};
+
+template <typename T> struct RnIo;
+template <> struct RnIo<float> {
+    static __device__ __forceinline__ f32x4 load(const void* p, long i) { return reinterpret_cast<const f32x4*>(p)[i]; }
+    static __device__ __forceinline__ void store(void* p, long i, f32x4 v) { reinterpret_cast<f32x4*>(p)[i] = v; }
+};
+template <> struct RnIo<bf16_t> {
+    static __device__ __forceinline__ f32x4 load(const void* p, long i) {
+        const uint2 w = reinterpret_cast<const uint2*>(p)[i];
+        return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                     __uint_as_float(w.y & 0xffff0000u)};
+    }
+    static __device__ __forceinline__ void store(void* p, long i, f32x4 v) {
+        reinterpret_cast<uint2*>(p)[i] = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+    }
+};
+
+// rows of one team: [lo, hi) of the rows that belong to a group (all, without cu)
+struct RnRun { long lo, hi, used; };
+__device__ __forceinline__ long rn_used(const RnArgs& a) {
+    if (!a.cu) return a.rows;
+    const int u = a.cu[a.groups];
+    return u < 0 ? 0 : u > a.rows ? a.rows : u;
+}
+__device__ __forceinline__ RnRun rn_run(const RnArgs& a, int team) {
+    const long used = rn_used(a);
+    return RnRun{used * team / a.teams, used * (team + 1) / a.teams, used};
+}
+// first row behind group g; the last group ends with the rows
+__device__ __forceinline__ long rn_group_end(const RnArgs& a, int g, long used) {
+    if (g >= a.groups - 1) return used;
+    const long e = a.cu ? (long)a.cu[g + 1] : (long)(a.rows / a.groups) * (g + 1);
+    return e < used ? e : used;
+}
+// the group of a row: the first one that ends behind it
+__device__ __forceinline__ int rn_group(const RnArgs& a, long row, long used) {
+    if (!a.cu) return (int)(row / (a.rows / a.groups));
+    int lo = 0, hi = a.groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (rn_group_end(a, mid, used) > row) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+// sums over a team; teams of several waves meet in LDS, two places in turn, so that one barrier a sum is enough
+template <int WPR>
+struct RnTeam {
+    float (*red)[2][4];
+    int turn;
+    __device__ __forceinline__ void sum2(float& p, float& q) {
+        p = row_sum(p);
+        q = row_sum(q);
+        p = (lane_f(p, 0) + lane_f(p, 16)) + (lane_f(p, 32) + lane_f(p, 48));
+        q = (lane_f(q, 0) + lane_f(q, 16)) + (lane_f(q, 32) + lane_f(q, 48));
+        if constexpr (WPR > 1) {
+            const int wave = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) {
+                red[turn][0][wave] = p;
+                red[turn][1][wave] = q;
+            }
+            __syncthreads();
+            p = q = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) {
+                p += red[turn][0][w];
+                q += red[turn][1][w];
+            }
+            turn ^= 1;
+        }
+    }
+    __device__ __forceinline__ float sum(float p) {
+        float q = 0.f;
+        sum2(p, q);
+        return p;
+    }
+};
+
+#define RN_EACH(i, c) \
+    _Pragma("unroll") for (int i = 0; i < NCH; ++i) \
+        if (const int c = lane + 64 * WPR * i; c < nch)
+
+// uh in place of u; (mean, 1/deviation) of the row
+template <int WPR, int NCH>
+__device__ __forceinline__ float2 rn_unit(f32x4 (&u)[NCH], int lane, int nch, float inv, float eps, int rms, RnTeam<WPR>& team) {
+    float mu = 0.f;
+    if (!rms) {
+        float s = 0.f;
+        RN_EACH(i, c) s += (u[i][0] + u[i][1]) + (u[i][2] + u[i][3]);
+        mu = team.sum(s) * inv;
+    }
+    float q = 0.f;
+    RN_EACH(i, c) {
+        u[i] -= mu;
+        q += (u[i][0] * u[i][0] + u[i][1] * u[i][1]) + (u[i][2] * u[i][2] + u[i][3] * u[i][3]);
+    }
+    const float r = rsqrtf(team.sum(q) * inv + eps);
+    RN_EACH(i, c) u[i] *= r;
+    return make_float2(mu, r);
+}
+
+template <typename T, int WPR, int NCH, bool POST>
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR) void res_norm_fwd_kernel(RnArgs a) {
+    __shared__ float red[2][2][4];
+    RnTeam<WPR> sums{red, 0};
+    const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int team = WPR == 1 ? blockIdx.x * RN_FWD_WAVES + (threadIdx.x >> 6) : blockIdx.x;
+    const int nch = a.cols >> 2;
+    const float inv = 1.f / (float)a.cols;
+    const RnRun run = rn_run(a, team);
+    const f32x4 one = {1.f, 1.f, 1.f, 1.f}, none = {0.f, 0.f, 0.f, 0.f};
+    f32x4 w1[NCH], b1[NCH], w2[NCH], b2[NCH], f[NCH];
+    RN_EACH(i, c) {
+        w2[i] = RnIo<float>::load(a.pre_w, c);
+        b2[i] = a.pre_b ? RnIo<float>::load(a.pre_b, c) : none;
+        f[i] = a.scale ? RnIo<float>::load(a.scale, c) : one;
+        if constexpr (POST) {
+            w1[i] = RnIo<float>::load(a.post_w, c);
+            b1[i] = a.post_b ? RnIo<float>::load(a.post_b, c) : none;
+        }
+    }
+    int g = 0;
+    long end = run.used;
+    for (long row = run.lo; row < run.hi; ++row) {
+        const long base = row * nch;
+        f32x4 x[NCH], h[NCH];
+        RN_EACH(i, c) {
+            x[i] = RnIo<float>::load(a.x, base + c);
+            h[i] = RnIo<T>::load(a.h, base + c);
+        }
+        if (a.gate && (row == run.lo || row >= end)) {
+            if (row == run.lo) {
+                g = rn_group(a, row, run.used);
+            } else {
+                do ++g; while (rn_group_end(a, g, run.used) <= row && g < a.groups - 1);
+            }
+            end = rn_group_end(a, g, run.used);
+            RN_EACH(i, c) {
+                f[i] = RnIo<float>::load(a.gate, (long)g * nch + c);
+                if (a.scale) f[i] *= RnIo<float>::load(a.scale, c);
+            }
+        }
+        float2 s1 = make_float2(0.f, 1.f);
+        if constexpr (POST) {
+            s1 = rn_unit<WPR, NCH>(h, lane, nch, inv, a.eps, a.rms, sums);
+            RN_EACH(i, c) h[i] = h[i] * w1[i] + b1[i];
+        }
+        RN_EACH(i, c) {
+            x[i] += h[i] * f[i];
+            RnIo<float>::store(a.x_out, base + c, x[i]);
+        }
+        const float2 s2 = rn_unit<WPR, NCH>(x, lane, nch, inv, a.eps, a.rms, sums);
+        RN_EACH(i, c) RnIo<T>::store(a.y, base + c, x[i] * w2[i] + b2[i]);
+        if (a.stats && lane == 0) {
+            a.stats[row] = s1.x;
+            a.stats[(long)a.rows + row] = s1.y;
+            a.stats[2L * a.rows + row] = s2.x;
+            a.stats[3L * a.rows + row] = s2.y;
+        }
+    }
+    if (a.zero_rest) {                                    // rows behind the last group, in outputs that nobody has filled
+        for (long row = run.used + team; row < a.rows; row += a.teams) {
+            RN_EACH(i, c) {
+                if (a.zero_rest & 1) RnIo<float>::store(a.x_out, row * nch + c, none);
+                if (a.zero_rest & 2) RnIo<T>::store(a.y, row * nch + c, none);
+            }
+        }
+    }
+}
+
+template <typename T, int WPR, int NCH, bool POST>
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_norm_bwd_kernel(RnArgs a) {
+    constexpr int TEAMS = WPR == 1 ? RN_BWD_WAVES : 1;
+    __shared__ float red[2][2][4];
+    RnTeam<WPR> sums{red, 0};
+    const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int team = blockIdx.x * TEAMS + (WPR == 1 ? threadIdx.x >> 6 : 0);
+    const int nch = a.cols >> 2;
+    const float inv = 1.f / (float)a.cols;
+    const RnRun run = rn_run(a, team);
+    const f32x4 one = {1.f, 1.f, 1.f, 1.f}, none = {0.f, 0.f, 0.f, 0.f};
+    const bool scaled = a.scale || a.gate;
+    f32x4 w1[NCH], b1[NCH], w2[NCH], f[NCH];
+    f32x4 sum[RN_SUMS][NCH], own[NCH];                    // own: the current group's sum of e n
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        own[i] = none;
+#pragma unroll
+        for (int k = 0; k < RN_SUMS; ++k) sum[k][i] = none;
+    }
+    RN_EACH(i, c) {
+        w2[i] = RnIo<float>::load(a.pre_w, c);
+        f[i] = a.scale ? RnIo<float>::load(a.scale, c) : one;
+        if constexpr (POST) {
+            w1[i] = RnIo<float>::load(a.post_w, c);
+            b1[i] = a.post_b ? RnIo<float>::load(a.post_b, c) : none;
+        }
+    }
+    int g = 0;
+    long end = run.used;
+    for (long row = run.lo; row < run.hi; ++row) {
+        const long base = row * nch;
+        f32x4 d[NCH], x[NCH], e[NCH], h[NCH];
+        RN_EACH(i, c) {
+            d[i] = RnIo<T>::load(a.dy, base + c);
+            x[i] = RnIo<float>::load(a.x, base + c);
+            e[i] = a.dres ? RnIo<float>::load(a.dres, base + c) : none;
+            h[i] = RnIo<T>::load(a.h, base + c);
+        }
+        const float mu1 = a.stats[row], r1 = a.stats[(long)a.rows + row];
+        const float mu2 = a.stats[2L * a.rows + row], r2 = a.stats[3L * a.rows + row];
+        if (a.gate && (row == run.lo || row >= end)) {
+            if (row == run.lo) {
+                g = rn_group(a, row, run.used);
+            } else {
+                RN_EACH(i, c) {
+                    RnIo<float>::store(a.slots, (long)(team + g) * nch + c, own[i]);
+                    sum[4][i] += own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
+                    own[i] = none;
+                }
+                do ++g; while (rn_group_end(a, g, run.used) <= row && g < a.groups - 1);
+            }
+            end = rn_group_end(a, g, run.used);
+            RN_EACH(i, c) {
+                f[i] = RnIo<float>::load(a.gate, (long)g * nch + c);
+                if (a.scale) f[i] *= RnIo<float>::load(a.scale, c);
+            }
+        }
+        float p = 0.f, q = 0.f;
+        RN_EACH(i, c) {
+            x[i] = (x[i] - mu2) * r2;
+            sum[0][i] += d[i] * x[i];
+            sum[1][i] += d[i];
+            d[i] *= w2[i];
+            p += (d[i][0] + d[i][1]) + (d[i][2] + d[i][3]);
+            q += (d[i][0] * x[i][0] + d[i][1] * x[i][1]) + (d[i][2] * x[i][2] + d[i][3] * x[i][3]);
+        }
+        sums.sum2(p, q);
+        p = a.rms ? 0.f : p * inv;
+        q *= inv;
+        RN_EACH(i, c) {
+            e[i] += (d[i] - p - x[i] * q) * r2;
+            RnIo<float>::store(a.dx, base + c, e[i]);
+        }
+        if constexpr (POST) {
+            p = q = 0.f;
+            RN_EACH(i, c) {
+                h[i] = (h[i] - mu1) * r1;
+                if (scaled) own[i] += e[i] * (h[i] * w1[i] + b1[i]);
+                e[i] *= f[i];
+                sum[2][i] += e[i] * h[i];
+                sum[3][i] += e[i];
+                e[i] *= w1[i];
+                p += (e[i][0] + e[i][1]) + (e[i][2] + e[i][3]);
+                q += (e[i][0] * h[i][0] + e[i][1] * h[i][1]) + (e[i][2] * h[i][2] + e[i][3] * h[i][3]);
+            }
+            sums.sum2(p, q);
+            p = a.rms ? 0.f : p * inv;
+            q *= inv;
+            RN_EACH(i, c) RnIo<T>::store(a.dh, base + c, (e[i] - p - h[i] * q) * r1);
+        } else {
+            RN_EACH(i, c) {
+                if (scaled) own[i] += e[i] * h[i];
+                RnIo<T>::store(a.dh, base + c, e[i] * f[i]);
+            }
+        }
+    }
+    if (a.gate) {
+        if (run.hi > run.lo) {
+            RN_EACH(i, c) {
+                RnIo<float>::store(a.slots, (long)(team + g) * nch + c, own[i]);
+                sum[4][i] += own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
+            }
+        }
+    } else {
+        RN_EACH(i, c) sum[4][i] = own[i];
+    }
+    if (a.zero_rest) {
+        for (long row = run.used + team; row < a.rows; row += a.teams) {
+            RN_EACH(i, c) {
+                if (a.zero_rest & 1) RnIo<float>::store(a.dx, row * nch + c, none);
+                if (a.zero_rest & 2) RnIo<T>::store(a.dh, row * nch + c, none);
+            }
+        }
+    }
+    // the workgroup's column sums, one kind after the other
+    float* part = a.part + (long)blockIdx.x * RN_SUMS * a.cols;
+    if constexpr (TEAMS == 1) {
+#pragma unroll
+        for (int k = 0; k < RN_SUMS; ++k) RN_EACH(i, c) RnIo<float>::store(part, (long)k * nch + c, sum[k][i]);
+    } else {
+        extern __shared__ __attribute__((aligned(16))) float lds[];                 // [TEAMS][cols]
+        f32x4* rows = reinterpret_cast<f32x4*>(lds);
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int k = 0; k < RN_SUMS; ++k) {
+            __syncthreads();
+            RN_EACH(i, c) rows[wave * nch + c] = sum[k][i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < nch; c += 64 * TEAMS) {
+                f32x4 s = rows[c];
+#pragma unroll
+                for (int w = 1; w < TEAMS; ++w) s += rows[w * nch + c];
+                RnIo<float>::store(part, (long)k * nch + c, s);
+            }
+        }
+    }
+}
+
+// Second launch of the backward pass: column sums over workgroups, and each group's slots.  64 columns x 16 slices.
+constexpr int RNF_SLICES = 16;
+struct RnOut { float* col[RN_SUMS]; float* gate; };
+__global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnArgs a, RnOut o, int blocks, int col_blocks,
+                                                                           int gate_rows) {
+    __shared__ float red[RNF_SLICES][64];
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int cb = cdiv_dev(a.cols, 64);
+    if ((int)blockIdx.x < col_blocks) {
+        const int k = blockIdx.x / cb, c = (blockIdx.x % cb) * 64 + lane;
+        if (!o.col[k]) return;
+        float s = 0.f;
+        if (c < a.cols)
+            for (int b = slice; b < blocks; b += RNF_SLICES) s += a.part[((long)b * RN_SUMS + k) * a.cols + c];
+        red[slice][lane] = s;
+        __syncthreads();
+        if (slice == 0 && c < a.cols) {
+            s = 0.f;
+#pragma unroll
+            for (int i = 0; i < RNF_SLICES; ++i) s += red[i][lane];
+            o.col[k][c] = s;
+        }
+        return;
+    }
+    // gate_rows == 1: 16 slices of one group's slots; else one group a slice
+    const int rest = blockIdx.x - col_blocks;
+    const int c = (rest % cb) * 64 + lane;
+    const int g = (rest / cb) * gate_rows + (gate_rows == 1 ? 0 : slice);
+    const long used = rn_used(a);
+    float s = 0.f;
+    if (g < a.groups && c < a.cols) {
+        const long lo = g == 0 ? 0 : rn_group_end(a, g - 1, used), hi = rn_group_end(a, g, used);
+        if (lo >= 0 && hi > lo) {
+            // the teams from the one with the first row to the one with the last; with fewer rows than teams most have none,
+            // and the rows' own teams are gone through
+            const bool few = used < a.teams;
+            const long w0 = ((lo + 1) * a.teams - 1) / used, n = few ? hi - lo : (hi * a.teams - 1) / used - w0 + 1;
+            for (long j = gate_rows == 1 ? slice : 0; j < n; j += gate_rows == 1 ? RNF_SLICES : 1) {
+                const long w = few ? ((lo + j + 1) * a.teams - 1) / used : w0 + j;
+                s += a.slots[(w + g) * a.cols + c];
+            }
+        }
+    }
+    if (gate_rows == 1) {
+        red[slice][lane] = s;
+        __syncthreads();
+        if (slice != 0) return;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < RNF_SLICES; ++i) s += red[i][lane];
+    }
+    if (g < a.groups && c < a.cols) o.gate[(long)g * a.cols + c] = a.scale ? s * a.scale[c] : s;
+}
+
+// waves of a team, and chunks a lane: columns over 64-lane waves of up to four 16-B chunks
+static void rn_shape(int cols, int* wpr, int* nch) {
+    *wpr = cols <= 1024 ? 1 : cols <= 2048 ? 2 : 4;
+    *nch = cdiv(cols / 4, 64 * *wpr);
+}
+static int rn_fwd_blocks(int rows, int cols) {
+    const int per = cols <= 1024 ? RN_FWD_WAVES : 1, most = cols <= 1024 ? 2048 : cols <= 2048 ? 4096 : 2048;
+    const int b = cdiv(rows, per);
+    return b < 1 ? 1 : b > most ? most : b;
+}
+static int rn_bwd_blocks(int rows, int cols) {
+    const int per = (cols <= 1024 ? RN_BWD_WAVES : 1) * 2, most = cols <= 1024 ? 512 : cols <= 2048 ? 1024 : 512;
+    const int b = cdiv(rows, per);
+    return b < 1 ? 1 : b > most ? most : b;
+}
+
+template <template <typename, int, int, bool> class Launch, typename T, bool POST>
+static int rn_pick2(int wpr, int nch, const RnArgs& a, int blocks, hipStream_t s) {
+    if (wpr == 1) {
+        switch (nch) {
+            case 1: return Launch<T, 1, 1, POST>::go(a, blocks, s);
+            case 2: return Launch<T, 1, 2, POST>::go(a, blocks, s);
+            case 3: return Launch<T, 1, 3, POST>::go(a, blocks, s);
+            default: return Launch<T, 1, 4, POST>::go(a, blocks, s);
+        }
+    }
+    if (wpr == 2) return nch == 3 ? Launch<T, 2, 3, POST>::go(a, blocks, s) : Launch<T, 2, 4, POST>::go(a, blocks, s);
+    return nch == 3 ? Launch<T, 4, 3, POST>::go(a, blocks, s) : Launch<T, 4, 4, POST>::go(a, blocks, s);
+}
+template <template <typename, int, int, bool> class Launch>
+static int rn_pick(int dtype, const RnArgs& a, int blocks, hipStream_t s) {
+    int wpr, nch;
+    rn_shape(a.cols, &wpr, &nch);
+    if (dtype == NEAT_F32)
+        return a.post_w ? rn_pick2<Launch, float, true>(wpr, nch, a, blocks, s) : rn_pick2<Launch, float, false>(wpr, nch, a, blocks, s);
+    return a.post_w ? rn_pick2<Launch, bf16_t, true>(wpr, nch, a, blocks, s) : rn_pick2<Launch, bf16_t, false>(wpr, nch, a, blocks, s);
+}
+template <typename T, int WPR, int NCH, bool POST> struct RnForward {
+    static int go(const RnArgs& a, int blocks, hipStream_t s) {
+        hipLaunchKernelGGL((res_norm_fwd_kernel<T, WPR, NCH, POST>), dim3(blocks),
+                           dim3(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR), 0, s, a);
+        NEAT_LAUNCH_CHECK("neat_res_norm_fwd");
+        return NEAT_OK;
+    }
+};
+template <typename T, int WPR, int NCH, bool POST> struct RnBackward {
+    static int go(const RnArgs& a, int blocks, hipStream_t s) {
+        const size_t lds = WPR == 1 ? (size_t)RN_BWD_WAVES * a.cols * 4 : 0;
+        hipLaunchKernelGGL((res_norm_bwd_kernel<T, WPR, NCH, POST>), dim3(blocks),
+                           dim3(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR), lds, s, a);
+        NEAT_LAUNCH_CHECK("neat_res_norm_bwd");
+        return NEAT_OK;
+    }
+};
+
+static bool rn_aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+static int rn_check(const char* who, const RnArgs& a, int dtype, int kind) {
+    NEAT_REQUIRE(dtype == NEAT_F32 || dtype == NEAT_BF16, NEAT_ERR_ARG, "%s: dtype=%d", who, dtype);
+    NEAT_REQUIRE(kind == NEAT_NORM_LAYER || kind == NEAT_NORM_RMS, NEAT_ERR_ARG, "%s: kind=%d", who, kind);
+    NEAT_REQUIRE(a.rows >= 0 && a.cols > 0 && a.cols % 4 == 0 && a.cols <= RN_MAX_COLS, NEAT_ERR_SHAPE,
+                 "%s: rows=%d cols=%d unsupported (cols %% 4 == 0, <= %d)", who, a.rows, a.cols, RN_MAX_COLS);
+    NEAT_REQUIRE(a.groups >= 0 && (a.gate == nullptr) == (a.groups == 0), NEAT_ERR_ARG, "%s: groups=%d need a gate each", who, a.groups);
+    NEAT_REQUIRE(!a.cu || a.gate, NEAT_ERR_ARG, "%s: cu without a gate", who);
+    NEAT_REQUIRE(!a.gate || a.cu || a.rows % a.groups == 0, NEAT_ERR_SHAPE, "%s: rows=%d do not divide into %d groups", who,
+                 a.rows, a.groups);
+    NEAT_REQUIRE(!a.post_b || a.post_w, NEAT_ERR_ARG, "%s: post_b without post_w", who);
+    for (const void* p : {(const void*)a.x, (const void*)a.pre_w, (const void*)a.pre_b, (const void*)a.post_w,
+                          (const void*)a.post_b, (const void*)a.scale, (const void*)a.gate, (const void*)a.x_out,
+                          (const void*)a.dres, (const void*)a.dx, (const void*)a.part})
+        NEAT_REQUIRE(rn_aligned(p, 16), NEAT_ERR_ARG, "%s: a float32 array is not 16-byte aligned", who);
+    for (const void* p : {a.h, (const void*)a.y, a.dy, (const void*)a.dh})
+        NEAT_REQUIRE(rn_aligned(p, dtype == NEAT_F32 ? 16 : 8), NEAT_ERR_ARG, "%s: an activation is not aligned to four elements", who);
+    return NEAT_OK;
+}
+
+}  // namespace neat
+
+using namespace neat;
+
+extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const float* pre_w, const float* pre_b,
+                                 const float* post_w, const float* post_b, const float* scale, const float* gate, int groups,
+                                 const int32_t* cu, float* x_out, void* y, float* stats, int zero_rest, int rows, int cols,
+                                 float eps, void* stream) {
+    RnArgs a{};
+    a.x = x; a.h = h; a.pre_w = pre_w; a.pre_b = pre_b; a.post_w = post_w; a.post_b = post_b; a.scale = scale; a.gate = gate;
+    a.groups = groups; a.cu = cu; a.x_out = x_out; a.y = y; a.stats = stats; a.zero_rest = zero_rest; a.rows = rows; a.cols = cols;
+    a.rms = kind == NEAT_NORM_RMS; a.eps = eps;
+    if (int rc = rn_check("neat_res_norm_fwd", a, dtype, kind)) return rc;
+    if (rows == 0) return NEAT_OK;
+    NEAT_REQUIRE(x && h && pre_w && x_out && y, NEAT_ERR_ARG, "neat_res_norm_fwd: null pointer");
+    const int blocks = rn_fwd_blocks(rows, cols);
+    a.teams = blocks * (cols <= 1024 ? RN_FWD_WAVES : 1);
+    return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
+}
+
+extern "C" long neat_res_norm_ws_floats(int rows, int cols, int groups) {
+    if (rows < 0 || cols <= 0 || cols > RN_MAX_COLS || groups < 0) return 0;
+    const long blocks = rn_bwd_blocks(rows, cols), teams = blocks * (cols <= 1024 ? RN_BWD_WAVES : 1);
+    return blocks * RN_SUMS * cols + (groups ? (teams + groups) * cols : 0);
+}
+
+extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* h, const float* x_out, const float* stats, int dtype,
+                                 int kind, const float* pre_w, const float* post_w, const float* post_b, const float* scale,
+                                 const float* gate, int groups, const int32_t* cu, float* dx, void* dh, float* dpre_w,
+                                 float* dpre_b, float* dpost_w, float* dpost_b, float* dscale, float* dgate, float* ws,
+                                 int zero_rest, int rows, int cols, void* stream) {
+    RnArgs a{};
+    a.dy = dy; a.dres = dres; a.h = h; a.x = x_out; a.stats = const_cast<float*>(stats); a.pre_w = pre_w; a.post_w = post_w;
+    a.post_b = post_b; a.scale = scale; a.gate = gate; a.groups = groups; a.cu = cu; a.dx = dx; a.dh = dh; a.part = ws;
+    a.zero_rest = zero_rest; a.rows = rows; a.cols = cols; a.rms = kind == NEAT_NORM_RMS;
+    if (int rc = rn_check("neat_res_norm_bwd", a, dtype, kind)) return rc;
+    NEAT_REQUIRE((dy && h && x_out && stats && dx && dh) || rows == 0, NEAT_ERR_ARG, "neat_res_norm_bwd: null pointer");
+    NEAT_REQUIRE(pre_w && ws, NEAT_ERR_ARG, "neat_res_norm_bwd: null pointer");
+    NEAT_REQUIRE((!dpost_w && !dpost_b) || post_w, NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a norm that is not there");
+    NEAT_REQUIRE((!dscale || scale) && (!dgate || gate), NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a scale or gate that is not there");
+    const int blocks = rn_bwd_blocks(rows, cols);
+    a.teams = blocks * (cols <= 1024 ? RN_BWD_WAVES : 1);
+    a.slots = gate ? ws + (long)blocks * RN_SUMS * cols : nullptr;
+    hipStream_t s = (hipStream_t)stream;
+    if (int rc = rn_pick<RnBackward>(dtype, a, blocks, s)) return rc;
+    const RnOut o{{dpre_w, dpre_b, dpost_w, dpost_b, dscale}, dgate};
+    const int cb = cdiv(cols, 64);
+    // few groups with many slots each: 16 slices a group; many groups: one slice each
+    const int gate_rows = groups > 0 && a.teams / groups >= 8 ? 1 : RNF_SLICES;
+    const int col_blocks = RN_SUMS * cb, gate_blocks = dgate ? cb * cdiv(groups, gate_rows) : 0;
+    hipLaunchKernelGGL(res_norm_finalize_kernel, dim3(col_blocks + gate_blocks), dim3(64 * RNF_SLICES), 0, s, a, o, blocks,
+                       col_blocks, gate_rows);
+    NEAT_LAUNCH_CHECK("neat_res_norm_bwd (sums)");
+    return NEAT_OK;
+}

@@ -13,6 +13,7 @@ LIB_PATH = os.environ.get("NEAT_HIP_LIB") or os.path.join(_HERE, "libneat_hip.so
 
 EPI_BF16, EPI_BIAS_BF16, EPI_BIAS_RES_F32, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_F32 = range(6)
 DT_F32, DT_BF16 = range(2)
+NORM_LAYER, NORM_RMS = range(2)
 
 _P, _I, _L, _F, _D = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_double
 
@@ -25,6 +26,10 @@ SIGNATURES = {
     "neat_ln_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
     "neat_ln_bwd_finalize": (_I, [_P, _I, _I, _P, _P, _I, _P]),
     "neat_ln_bwd_finalize_batched": (_I, [_P, _I, _I, _I, _P, _I, _P]),
+    "neat_res_norm_fwd": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
+    "neat_res_norm_ws_floats": (_L, [_I, _I, _I]),
+    "neat_res_norm_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I,
+                               _P]),
     "neat_pack_weight_bf16": (_I, [_P, _P, _I, _I, _I, _P]),
     "neat_gemm_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "neat_pack_weight_bf16_t256": (_I, [_P, _P, _I, _I, _I, _P]),

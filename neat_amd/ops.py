@@ -91,6 +91,27 @@ def _p(t: Optional[torch.Tensor], dtype=None, name="tensor") -> Optional[int]:
     return t.data_ptr()
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+_DTYPES = {f32: lib.DT_F32, bf16: lib.DT_BF16}
+
+
+def _call_on(device, name, *args):
+    """lib.call with the current stream of ``device``, which is made current where it is not (the library launches on the
+    current device)."""
+    if device.index == _device_index():
+        lib.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            lib.call(name, *args, _stream())
+
+
+def _device_index() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
 # ---- LayerNorm ----
 def ln_fwd(x, gamma, beta, eps=1e-5, out_bf16=True, out_f32=False, save_stats=True):
     rows, cols = x.numel() // x.shape[-1], x.shape[-1]
@@ -154,6 +175,93 @@ def ln_bwd_finalize_batched(partials, dsts, accumulate=False):
         _PTR_TABLES[key] = table
     lib.call("neat_ln_bwd_finalize_batched", _p(partials, f32, "partials"), nblk, cols, count, _p(table), int(accumulate),
              _stream())
+
+
+# ---- the norms around a block with its gate and residual scale ----
+_NORMS = {"ln": lib.NORM_LAYER, "rms": lib.NORM_RMS}
+
+
+def _res_norm_args(who, x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu, kind):
+    """Checks what both directions share -> (rows, cols, groups, dtype, kind, device)."""
+    if kind not in _NORMS:
+        raise RuntimeError(f"{who}: kind must be 'ln' or 'rms', got {kind!r}")
+    if x.dim() != 2 or h.shape != x.shape or h.dtype not in _DTYPES:
+        raise RuntimeError(f"{who}: expected [rows, cols], float32 stream and float32 or bfloat16 branch, got "
+                           f"{tuple(x.shape)} and {h.dtype} {tuple(h.shape)}")
+    rows, cols = x.shape
+    for t, nm in ((pre_w, "pre_w"), (pre_b, "pre_b"), (post_w, "post_w"), (post_b, "post_b"), (scale, "scale")):
+        if t is not None and (tuple(t.shape) != (cols,) or t.device != x.device):
+            raise RuntimeError(f"{who}: {nm} must be float32 [{cols}] on the stream's device")
+    if post_b is not None and post_w is None:
+        raise RuntimeError(f"{who}: post_b without post_w")
+    groups = 0
+    if gate is not None:
+        groups = gate.shape[0]
+        if gate.dim() != 2 or gate.shape[1] != cols or groups < 1 or gate.device != x.device:
+            raise RuntimeError(f"{who}: gate must be float32 [groups, {cols}] on the stream's device")
+        if cu is None and rows % groups:
+            raise RuntimeError(f"{who}: {rows} rows do not divide into {groups} groups (pass cu)")
+    if cu is not None and (gate is None or tuple(cu.shape) != (groups + 1,) or cu.device != x.device):
+        raise RuntimeError(f"{who}: cu must be int32 [groups + 1] beside a gate")
+    return rows, cols, groups, _DTYPES[h.dtype], _NORMS[kind], x.device
+
+
+def _res_norm_out(t, like, dtype, who):
+    """(tensor, whether rows behind the last group are to be zeroed: in a buffer made here they hold nothing)."""
+    if t is None:
+        return torch.empty(like.shape, dtype=dtype, device=like.device), True
+    if t.shape != like.shape or t.device != like.device:
+        raise RuntimeError(f"{who}: an output has another shape or device than its input")
+    return t, False
+
+
+def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, gate=None, cu=None, kind="ln", eps=1e-5, save=True,
+                 x_out=None, y=None):
+    """One junction between two blocks of a tower: the residual stream x (float32 [rows, cols]) takes the branch h (float32
+    or bfloat16), normed behind its block (``post_w``, ``post_b``; None: as it is), times ``scale`` [cols] and the ``gate``
+    [groups, cols] of its row's group, and is normed for the next block (``pre_w``, ``pre_b``):
+    x_out = x + N_post(h) * scale * gate, y = N_pre(x_out) -> (x_out, y in h's type, stats for ``res_norm_bwd`` or None).
+    ``kind``: "ln" or "rms".  Groups are rows // groups rows each, or the sequences of a packed batch (``cu`` int32 [groups
+    + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (x_out may be x), zero in new ones."""
+    rows, cols, groups, dt, kd, dev = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu, kind)
+    x_out, zx = _res_norm_out(x_out, x, f32, "res_norm_fwd")
+    y, zy = _res_norm_out(y, h, h.dtype, "res_norm_fwd")
+    stats = torch.empty(4, rows, dtype=f32, device=dev) if save else None
+    _call_on(dev, "neat_res_norm_fwd", _p(x, f32, "x"), _p(h, None, "h"), dt, kd, _p(pre_w, f32, "pre_w"), _p(pre_b, f32, "pre_b"),
+             _p(post_w, f32, "post_w"), _p(post_b, f32, "post_b"), _p(scale, f32, "scale"), _p(gate, f32, "gate"), groups,
+             _p(cu, i32, "cu"), _p(x_out, f32, "x_out"), _p(y, h.dtype, "y"), _ptr(stats),
+             (int(zx) | 2 * int(zy)) if cu is not None else 0, rows, cols, float(eps))
+    return x_out, y, stats
+
+
+@functools.lru_cache(maxsize=256)
+def _res_norm_ws_floats(rows, cols, groups):
+    return lib.load().neat_res_norm_ws_floats(rows, cols, groups)
+
+
+def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, scale=None, gate=None, cu=None, kind="ln", dx=None,
+                 dh=None):
+    """Backward of ``res_norm_fwd``: dy = gradient of y (h's type), dres = gradient of x_out from elsewhere (float32 or None) ->
+    (dx float32, dh in h's type, {"pre_w", "pre_b", "post_w", "post_b", "scale", "gate"}: float32 gradients of what was given;
+    those of a bias are there with their weight's).  ``dx`` may be dres.  Sums are formed in a fixed order."""
+    rows, cols, groups, dt, kd, dev = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu, kind)
+    if dy.shape != h.shape or dy.device != dev or tuple(stats.shape) != (4, rows) or stats.device != dev:
+        raise RuntimeError("res_norm_bwd: dy must have the branch's shape and stats be the forward pass's [4, rows]")
+    if dres is not None and (dres.shape != x_out.shape or dres.device != dev):
+        raise RuntimeError("res_norm_bwd: dres must have the stream's shape")
+    dx, zx = _res_norm_out(dx, x_out, f32, "res_norm_bwd")
+    dh, zh = _res_norm_out(dh, h, h.dtype, "res_norm_bwd")
+    names = ["pre_w", "pre_b"] + (["post_w", "post_b"] if post_w is not None else []) + (["scale"] if scale is not None else [])
+    grads = dict(zip(names, torch.empty(len(names), cols, dtype=f32, device=dev).unbind(0)))
+    if gate is not None:
+        grads["gate"] = torch.empty(groups, cols, dtype=f32, device=dev)
+    ws = torch.empty(_res_norm_ws_floats(rows, cols, groups), dtype=f32, device=dev)
+    g = [_ptr(grads.get(n)) for n in ("pre_w", "pre_b", "post_w", "post_b", "scale", "gate")]
+    _call_on(dev, "neat_res_norm_bwd", _p(dy, h.dtype, "dy"), _p(dres, f32, "dres"), _p(h, None, "h"), _p(x_out, f32, "x_out"),
+             _p(stats, f32, "stats"), dt, kd, _p(pre_w, f32, "pre_w"), _p(post_w, f32, "post_w"), _p(post_b, f32, "post_b"),
+             _p(scale, f32, "scale"), _p(gate, f32, "gate"), groups, _p(cu, i32, "cu"), _p(dx, f32, "dx"), _p(dh, h.dtype, "dh"),
+             *g, ws.data_ptr(), (int(zx) | 2 * int(zh)) if cu is not None else 0, rows, cols)
+    return dx, dh, grads
 
 
 # ---- GEMM ----
@@ -521,22 +629,7 @@ def adamw_flat(p, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.0):
              float(beta1), float(beta2), float(eps), float(wd), int(step), _stream())
 
 
-def _call_on(device, name, *args):
-    """lib.call with the current stream of ``device``, which is made current where it is not (the library launches on the
-    current device)."""
-    if device.index == _device_index():
-        lib.call(name, *args, _stream())
-    else:
-        with torch.cuda.device(device):
-            lib.call(name, *args, _stream())
-
-
-def _device_index() -> int:
-    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
-
-
 ADAMW_BLOCK = 256            # elements of one tensor that share a block of moments (and, in 8 bits, a scale)
-_DTYPES = {f32: lib.DT_F32, bf16: lib.DT_BF16}
 
 
 def adamw_multi(params, grads, state_blocks, steps, m, v, m_scale=None, v_scale=None, lr=1e-3, beta1=0.9, beta2=0.999,
@@ -752,8 +845,6 @@ def _lp_ws(dtype, R, V, k, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _lp_out(out, logits):

@@ -97,3 +97,36 @@ def test_token_logprobs_wrapper_refuses():
                  lambda: ops.token_logprobs_bwd(z, None, torch.zeros(3, 3)), lambda: ops.token_logprobs_fwd_bwd(z, None)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def _rn(x=64, h=64, dtype=0, kind=0, pre_w=64, pre_b=64, post_w=64, post_b=64, scale=64, gate=64, groups=2, cu=None, x_out=64, y=64,
+        rows=4, cols=64):
+    return lib.load().neat_res_norm_fwd(x, h, dtype, kind, pre_w, pre_b, post_w, post_b, scale, gate, groups, cu, x_out, y, 64, 0, rows,
+                                        cols, 1e-5, None)
+
+
+@pytest.mark.parametrize("bad, rc, says", [
+    (dict(x=None), -2, "null"), (dict(h=None), -2, "null"), (dict(pre_w=None), -2, "null"), (dict(y=None), -2, "null"),
+    (dict(dtype=5), -2, "dtype"), (dict(kind=2), -2, "kind"), (dict(cols=66), -1, "cols"), (dict(cols=4100), -1, "cols"),
+    (dict(rows=-1), -1, "rows"), (dict(rows=5), -1, "divide"), (dict(groups=0), -2, "groups"), (dict(gate=None), -2, "groups"),
+    (dict(gate=None, groups=0, cu=64), -2, "cu"), (dict(post_w=None), -2, "post_b"), (dict(x=72), -2, "aligned"),
+    (dict(h=72), -2, "aligned"), (dict(h=68, dtype=1), -2, "aligned"), (dict(scale=68), -2, "aligned")])
+def test_res_norm_checks_before_launching(bad, rc, says):
+    assert _rn(**bad) == rc
+    assert says in lib.last_error()
+
+
+def test_res_norm_backward_checks_before_launching():
+    L = lib.load()
+
+    def call(**k):
+        v = dict(dy=64, h=64, x_out=64, stats=64, post_w=64, scale=64, gate=64, groups=2, dpost_w=64, dscale=64, dgate=64, ws=64)
+        v.update(k)
+        return L.neat_res_norm_bwd(v["dy"], 64, v["h"], v["x_out"], v["stats"], 0, 0, 64, v["post_w"], None, v["scale"], v["gate"],
+                                   v["groups"], None, 64, 64, 64, 64, v["dpost_w"], None, v["dscale"], v["dgate"], v["ws"], 0, 4, 64,
+                                   None)
+    for bad in (dict(dy=None), dict(stats=None), dict(ws=None), dict(post_w=None), dict(scale=None), dict(gate=None, groups=0),
+                dict(ws=72)):
+        assert call(**bad) == -2, bad
+    assert L.neat_res_norm_ws_floats(4, 64, 2) > 5 * 64
+    assert _rn(rows=0) == 0
