@@ -21,7 +21,7 @@
 namespace neat {
 
 constexpr int RN_MAX_COLS = 4096;
-constexpr int RN_FWD_WAVES = 4, RN_BWD_WAVES = 8;         // waves of a workgroup whose teams are single waves
+constexpr int RN_FWD_WAVES = 4, RN_BWD_WAVES = 4;         // waves of a workgroup whose teams are single waves
 constexpr int RN_SUMS = 5;                                // column sums: pre_w, pre_b, post_w, post_b, scale
 
 struct RnArgs {
@@ -45,12 +45,17 @@ struct RnArgs {
 
 template <typename T> struct RnIo;
 template <> struct RnIo<float> {
+    typedef f32x4 raw;
+    static __device__ __forceinline__ raw fetch(const void* p, long i) { return reinterpret_cast<const f32x4*>(p)[i]; }
+    static __device__ __forceinline__ f32x4 open(raw w) { return w; }
     static __device__ __forceinline__ f32x4 load(const void* p, long i) { return reinterpret_cast<const f32x4*>(p)[i]; }
     static __device__ __forceinline__ void store(void* p, long i, f32x4 v) { reinterpret_cast<f32x4*>(p)[i] = v; }
 };
 template <> struct RnIo<bf16_t> {
-    static __device__ __forceinline__ f32x4 load(const void* p, long i) {
-        const uint2 w = reinterpret_cast<const uint2*>(p)[i];
+    typedef uint2 raw;
+    static __device__ __forceinline__ raw fetch(const void* p, long i) { return reinterpret_cast<const uint2*>(p)[i]; }
+    static __device__ __forceinline__ f32x4 load(const void* p, long i) { return open(fetch(p, i)); }
+    static __device__ __forceinline__ f32x4 open(raw w) {
         return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                      __uint_as_float(w.y & 0xffff0000u)};
     }
@@ -143,64 +148,90 @@ __device__ __forceinline__ float2 rn_unit(f32x4 (&u)[NCH], int lane, int nch, fl
     return make_float2(mu, r);
 }
 
+// weights in LDS, one copy a workgroup: they are read once a row from there, and the registers they would fill hold rows in
+// flight.  Zeros (ones) stand for what is not given.
+template <int THREADS>
+__device__ __forceinline__ void rn_stage(f32x4* dst, const float* src, float otherwise, int nch) {
+    for (int c = threadIdx.x; c < nch; c += THREADS)
+        dst[c] = src ? RnIo<float>::load(src, c) : f32x4{otherwise, otherwise, otherwise, otherwise};
+}
+
+// the factor of a row's branch: scale times its group's gate
+template <int WPR, int NCH>
+__device__ __forceinline__ void rn_factor(f32x4 (&f)[NCH], const RnArgs& a, int g, int lane, int nch) {
+    RN_EACH(i, c) {
+        f[i] = RnIo<float>::load(a.gate, (long)g * nch + c);
+        if (a.scale) f[i] *= RnIo<float>::load(a.scale, c);
+    }
+}
+__device__ __forceinline__ int rn_next_group(const RnArgs& a, int g, long row, long used) {
+    do ++g; while (rn_group_end(a, g, used) <= row && g < a.groups - 1);
+    return g;
+}
+
 template <typename T, int WPR, int NCH, bool POST>
-__global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR) void res_norm_fwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR, NCH <= 2 ? 7 : NCH <= 4 ? 4 : NCH <= 6 ? 3 : 2) void res_norm_fwd_kernel(RnArgs a) {
+    constexpr int THREADS = WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR;
     __shared__ float red[2][2][4];
+    extern __shared__ __attribute__((aligned(16))) f32x4 lds[];               // pre_w, pre_b, post_w, post_b: [4][cols]
     RnTeam<WPR> sums{red, 0};
     const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int team = WPR == 1 ? blockIdx.x * RN_FWD_WAVES + (threadIdx.x >> 6) : blockIdx.x;
+    const int team = WPR == 1 ? blockIdx.x * RN_FWD_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
     const int nch = a.cols >> 2;
     const float inv = 1.f / (float)a.cols;
     const RnRun run = rn_run(a, team);
     const f32x4 one = {1.f, 1.f, 1.f, 1.f}, none = {0.f, 0.f, 0.f, 0.f};
-    f32x4 w1[NCH], b1[NCH], w2[NCH], b2[NCH], f[NCH];
-    RN_EACH(i, c) {
-        w2[i] = RnIo<float>::load(a.pre_w, c);
-        b2[i] = a.pre_b ? RnIo<float>::load(a.pre_b, c) : none;
-        f[i] = a.scale ? RnIo<float>::load(a.scale, c) : one;
-        if constexpr (POST) {
-            w1[i] = RnIo<float>::load(a.post_w, c);
-            b1[i] = a.post_b ? RnIo<float>::load(a.post_b, c) : none;
+    f32x4 x[NCH], f[NCH];
+    typename RnIo<T>::raw hn[NCH];
+    if (run.lo < run.hi) {                                // the first row is under way while the weights are staged
+        RN_EACH(i, c) {
+            x[i] = RnIo<float>::load(a.x, run.lo * nch + c);
+            hn[i] = RnIo<T>::fetch(a.h, run.lo * nch + c);
         }
     }
-    int g = 0;
-    long end = run.used;
+    rn_stage<THREADS>(lds, a.pre_w, 1.f, nch);
+    rn_stage<THREADS>(lds + nch, a.pre_b, 0.f, nch);
+    if constexpr (POST) {
+        rn_stage<THREADS>(lds + 2 * nch, a.post_w, 1.f, nch);
+        rn_stage<THREADS>(lds + 3 * nch, a.post_b, 0.f, nch);
+    }
+    RN_EACH(i, c) f[i] = a.scale ? RnIo<float>::load(a.scale, c) : one;
+    __syncthreads();
+    int g = -1;
+    long end = a.gate ? run.lo : run.used;
     for (long row = run.lo; row < run.hi; ++row) {
         const long base = row * nch;
-        f32x4 x[NCH], h[NCH];
-        RN_EACH(i, c) {
-            x[i] = RnIo<float>::load(a.x, base + c);
-            h[i] = RnIo<T>::load(a.h, base + c);
-        }
-        if (a.gate && (row == run.lo || row >= end)) {
-            if (row == run.lo) {
-                g = rn_group(a, row, run.used);
-            } else {
-                do ++g; while (rn_group_end(a, g, run.used) <= row && g < a.groups - 1);
-            }
-            end = rn_group_end(a, g, run.used);
+        f32x4 h[NCH], xn[NCH];
+        RN_EACH(i, c) h[i] = RnIo<T>::open(hn[i]);
+        if (row + 1 < run.hi) {                           // the next row, while this one is worked on
             RN_EACH(i, c) {
-                f[i] = RnIo<float>::load(a.gate, (long)g * nch + c);
-                if (a.scale) f[i] *= RnIo<float>::load(a.scale, c);
+                xn[i] = RnIo<float>::load(a.x, base + nch + c);
+                hn[i] = RnIo<T>::fetch(a.h, base + nch + c);
             }
+        }
+        if (row >= end) {
+            g = g < 0 ? rn_group(a, row, run.used) : rn_next_group(a, g, row, run.used);
+            end = rn_group_end(a, g, run.used);
+            rn_factor<WPR, NCH>(f, a, g, lane, nch);
         }
         float2 s1 = make_float2(0.f, 1.f);
         if constexpr (POST) {
             s1 = rn_unit<WPR, NCH>(h, lane, nch, inv, a.eps, a.rms, sums);
-            RN_EACH(i, c) h[i] = h[i] * w1[i] + b1[i];
+            RN_EACH(i, c) h[i] = h[i] * lds[2 * nch + c] + lds[3 * nch + c];
         }
         RN_EACH(i, c) {
             x[i] += h[i] * f[i];
             RnIo<float>::store(a.x_out, base + c, x[i]);
         }
         const float2 s2 = rn_unit<WPR, NCH>(x, lane, nch, inv, a.eps, a.rms, sums);
-        RN_EACH(i, c) RnIo<T>::store(a.y, base + c, x[i] * w2[i] + b2[i]);
+        RN_EACH(i, c) RnIo<T>::store(a.y, base + c, x[i] * lds[c] + lds[nch + c]);
         if (a.stats && lane == 0) {
             a.stats[row] = s1.x;
             a.stats[(long)a.rows + row] = s1.y;
             a.stats[2L * a.rows + row] = s2.x;
             a.stats[3L * a.rows + row] = s2.y;
         }
+        RN_EACH(i, c) x[i] = xn[i];
     }
     if (a.zero_rest) {                                    // rows behind the last group, in outputs that nobody has filled
         for (long row = run.used + team; row < a.rows; row += a.teams) {
@@ -212,36 +243,43 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR) void res_n
     }
 }
 
+// the second bound: waves a SIMD, so that registers are not spent on scheduling what other waves hide anyway
 template <typename T, int WPR, int NCH, bool POST>
-__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_norm_bwd_kernel(RnArgs a) {
-    constexpr int TEAMS = WPR == 1 ? RN_BWD_WAVES : 1;
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, NCH == 1 ? 6 : NCH == 2 ? 4 : NCH == 3 ? 3 : 2) void res_norm_bwd_kernel(RnArgs a) {
+    constexpr int TEAMS = WPR == 1 ? RN_BWD_WAVES : 1, THREADS = 64 * WPR * TEAMS;
     __shared__ float red[2][2][4];
+    // pre_w, post_w, post_b: [3][cols]; behind them a team's sum of gate times group sums [TEAMS][cols]; at the end the sums
+    extern __shared__ __attribute__((aligned(16))) f32x4 lds[];
     RnTeam<WPR> sums{red, 0};
+    const int wave = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int team = blockIdx.x * TEAMS + (WPR == 1 ? threadIdx.x >> 6 : 0);
+    const int team = blockIdx.x * TEAMS + wave;
     const int nch = a.cols >> 2;
     const float inv = 1.f / (float)a.cols;
     const RnRun run = rn_run(a, team);
     const f32x4 one = {1.f, 1.f, 1.f, 1.f}, none = {0.f, 0.f, 0.f, 0.f};
     const bool scaled = a.scale || a.gate;
-    f32x4 w1[NCH], b1[NCH], w2[NCH], f[NCH];
-    f32x4 sum[RN_SUMS][NCH], own[NCH];                    // own: the current group's sum of e n
+    f32x4* gated = lds + (3 + wave) * nch;
+    rn_stage<THREADS>(lds, a.pre_w, 1.f, nch);
+    if constexpr (POST) {
+        rn_stage<THREADS>(lds + nch, a.post_w, 1.f, nch);
+        rn_stage<THREADS>(lds + 2 * nch, a.post_b, 0.f, nch);
+    }
+    f32x4 f[NCH];
+    f32x4 sum[4][NCH], own[NCH];                          // own: sum of e n over the current group (all rows, without a gate)
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         own[i] = none;
 #pragma unroll
-        for (int k = 0; k < RN_SUMS; ++k) sum[k][i] = none;
+        for (int k = 0; k < 4; ++k) sum[k][i] = none;
     }
     RN_EACH(i, c) {
-        w2[i] = RnIo<float>::load(a.pre_w, c);
         f[i] = a.scale ? RnIo<float>::load(a.scale, c) : one;
-        if constexpr (POST) {
-            w1[i] = RnIo<float>::load(a.post_w, c);
-            b1[i] = a.post_b ? RnIo<float>::load(a.post_b, c) : none;
-        }
+        if (a.gate) gated[c] = none;
     }
-    int g = 0;
-    long end = run.used;
+    __syncthreads();
+    int g = -1;
+    long end = a.gate ? run.lo : run.used;
     for (long row = run.lo; row < run.hi; ++row) {
         const long base = row * nch;
         f32x4 d[NCH], x[NCH], e[NCH], h[NCH];
@@ -253,29 +291,24 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_n
         }
         const float mu1 = a.stats[row], r1 = a.stats[(long)a.rows + row];
         const float mu2 = a.stats[2L * a.rows + row], r2 = a.stats[3L * a.rows + row];
-        if (a.gate && (row == run.lo || row >= end)) {
-            if (row == run.lo) {
-                g = rn_group(a, row, run.used);
-            } else {
+        if (row >= end) {
+            if (g >= 0) {
                 RN_EACH(i, c) {
                     RnIo<float>::store(a.slots, (long)(team + g) * nch + c, own[i]);
-                    sum[4][i] += own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
+                    gated[c] += own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
                     own[i] = none;
                 }
-                do ++g; while (rn_group_end(a, g, run.used) <= row && g < a.groups - 1);
             }
+            g = g < 0 ? rn_group(a, row, run.used) : rn_next_group(a, g, row, run.used);
             end = rn_group_end(a, g, run.used);
-            RN_EACH(i, c) {
-                f[i] = RnIo<float>::load(a.gate, (long)g * nch + c);
-                if (a.scale) f[i] *= RnIo<float>::load(a.scale, c);
-            }
+            rn_factor<WPR, NCH>(f, a, g, lane, nch);
         }
         float p = 0.f, q = 0.f;
         RN_EACH(i, c) {
             x[i] = (x[i] - mu2) * r2;
             sum[0][i] += d[i] * x[i];
             sum[1][i] += d[i];
-            d[i] *= w2[i];
+            d[i] *= lds[c];
             p += (d[i][0] + d[i][1]) + (d[i][2] + d[i][3]);
             q += (d[i][0] * x[i][0] + d[i][1] * x[i][1]) + (d[i][2] * x[i][2] + d[i][3] * x[i][3]);
         }
@@ -289,12 +322,13 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_n
         if constexpr (POST) {
             p = q = 0.f;
             RN_EACH(i, c) {
+                const f32x4 w1 = lds[nch + c];
                 h[i] = (h[i] - mu1) * r1;
-                if (scaled) own[i] += e[i] * (h[i] * w1[i] + b1[i]);
+                if (scaled) own[i] += e[i] * (h[i] * w1 + lds[2 * nch + c]);
                 e[i] *= f[i];
                 sum[2][i] += e[i] * h[i];
                 sum[3][i] += e[i];
-                e[i] *= w1[i];
+                e[i] *= w1;
                 p += (e[i][0] + e[i][1]) + (e[i][2] + e[i][3]);
                 q += (e[i][0] * h[i][0] + e[i][1] * h[i][1]) + (e[i][2] * h[i][2] + e[i][3] * h[i][3]);
             }
@@ -310,14 +344,12 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_n
         }
     }
     if (a.gate) {
-        if (run.hi > run.lo) {
+        if (g >= 0) {
             RN_EACH(i, c) {
                 RnIo<float>::store(a.slots, (long)(team + g) * nch + c, own[i]);
-                sum[4][i] += own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
+                own[i] = gated[c] + own[i] * RnIo<float>::load(a.gate, (long)g * nch + c);
             }
         }
-    } else {
-        RN_EACH(i, c) sum[4][i] = own[i];
     }
     if (a.zero_rest) {
         for (long row = run.used + team; row < a.rows; row += a.teams) {
@@ -331,20 +363,17 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR) void res_n
     float* part = a.part + (long)blockIdx.x * RN_SUMS * a.cols;
     if constexpr (TEAMS == 1) {
 #pragma unroll
-        for (int k = 0; k < RN_SUMS; ++k) RN_EACH(i, c) RnIo<float>::store(part, (long)k * nch + c, sum[k][i]);
+        for (int k = 0; k < RN_SUMS; ++k) RN_EACH(i, c) RnIo<float>::store(part, (long)k * nch + c, k < 4 ? sum[k & 3][i] : own[i]);
     } else {
-        extern __shared__ __attribute__((aligned(16))) float lds[];                 // [TEAMS][cols]
-        f32x4* rows = reinterpret_cast<f32x4*>(lds);
-        const int wave = threadIdx.x >> 6;
 #pragma unroll
         for (int k = 0; k < RN_SUMS; ++k) {
             __syncthreads();
-            RN_EACH(i, c) rows[wave * nch + c] = sum[k][i];
+            RN_EACH(i, c) lds[wave * nch + c] = k < 4 ? sum[k & 3][i] : own[i];
             __syncthreads();
-            for (int c = threadIdx.x; c < nch; c += 64 * TEAMS) {
-                f32x4 s = rows[c];
+            for (int c = threadIdx.x; c < nch; c += THREADS) {
+                f32x4 s = lds[c];
 #pragma unroll
-                for (int w = 1; w < TEAMS; ++w) s += rows[w * nch + c];
+                for (int w = 1; w < TEAMS; ++w) s += lds[w * nch + c];
                 RnIo<float>::store(part, (long)k * nch + c, s);
             }
         }
@@ -364,6 +393,7 @@ __global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnAr
         if (!o.col[k]) return;
         float s = 0.f;
         if (c < a.cols)
+#pragma unroll 8
             for (int b = slice; b < blocks; b += RNF_SLICES) s += a.part[((long)b * RN_SUMS + k) * a.cols + c];
         red[slice][lane] = s;
         __syncthreads();
@@ -388,6 +418,7 @@ __global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnAr
             // and the rows' own teams are gone through
             const bool few = used < a.teams;
             const long w0 = ((lo + 1) * a.teams - 1) / used, n = few ? hi - lo : (hi * a.teams - 1) / used - w0 + 1;
+#pragma unroll 4
             for (long j = gate_rows == 1 ? slice : 0; j < n; j += gate_rows == 1 ? RNF_SLICES : 1) {
                 const long w = few ? ((lo + j + 1) * a.teams - 1) / used : w0 + j;
                 s += a.slots[(w + g) * a.cols + c];
@@ -405,60 +436,84 @@ __global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnAr
     if (g < a.groups && c < a.cols) o.gate[(long)g * a.cols + c] = a.scale ? s * a.scale[c] : s;
 }
 
-// waves of a team, and chunks a lane: columns over 64-lane waves of up to four 16-B chunks
-static void rn_shape(int cols, int* wpr, int* nch) {
-    *wpr = cols <= 1024 ? 1 : cols <= 2048 ? 2 : 4;
-    *nch = cdiv(cols / 4, 64 * *wpr);
-}
+// waves of a team, and 16-B chunks a lane.  Forward a lane holds eight chunks of x and h without trouble; backward four, beside
+// five sums of them.
+static int rn_fwd_wpr(int cols) { return cols <= 2048 ? 1 : 2; }
+static int rn_bwd_wpr(int cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : 4; }
 static int rn_fwd_blocks(int rows, int cols) {
-    const int per = cols <= 1024 ? RN_FWD_WAVES : 1, most = cols <= 1024 ? 2048 : cols <= 2048 ? 4096 : 2048;
-    const int b = cdiv(rows, per);
+    const int per = rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1;
+    const int b = cdiv(rows, per * 4), most = 8192 / per;
     return b < 1 ? 1 : b > most ? most : b;
 }
 static int rn_bwd_blocks(int rows, int cols) {
-    const int per = (cols <= 1024 ? RN_BWD_WAVES : 1) * 2, most = cols <= 1024 ? 512 : cols <= 2048 ? 1024 : 512;
-    const int b = cdiv(rows, per);
+    const int per = rn_bwd_wpr(cols) == 1 ? RN_BWD_WAVES : 1, most = cols <= 1024 ? 768 : cols <= 2048 ? 1024 : 512;
+    const int b = cdiv(rows, per * 2);
     return b < 1 ? 1 : b > most ? most : b;
 }
 
-template <template <typename, int, int, bool> class Launch, typename T, bool POST>
-static int rn_pick2(int wpr, int nch, const RnArgs& a, int blocks, hipStream_t s) {
-    if (wpr == 1) {
-        switch (nch) {
-            case 1: return Launch<T, 1, 1, POST>::go(a, blocks, s);
-            case 2: return Launch<T, 1, 2, POST>::go(a, blocks, s);
-            case 3: return Launch<T, 1, 3, POST>::go(a, blocks, s);
-            default: return Launch<T, 1, 4, POST>::go(a, blocks, s);
+// dynamic LDS that any launch may have beside the static, and the most that is asked for (4 rows of 4 096 columns)
+constexpr size_t RN_PLAIN_LDS = 60 * 1024;
+constexpr int RN_MOST_LDS = 64 * 1024;
+template <typename T, bool POST> struct RnForward {
+    template <int WPR, int NCH> static int go(const RnArgs& a, int blocks, hipStream_t s) {
+        const size_t lds = (size_t)(POST ? 4 : 2) * a.cols * 4;
+        if (lds > RN_PLAIN_LDS) {
+            static unsigned long long done = 0;
+            if (int rc = ensure_dynamic_lds((const void*)res_norm_fwd_kernel<T, WPR, NCH, POST>, RN_MOST_LDS, &done, "neat_res_norm_fwd"))
+                return rc;
         }
-    }
-    if (wpr == 2) return nch == 3 ? Launch<T, 2, 3, POST>::go(a, blocks, s) : Launch<T, 2, 4, POST>::go(a, blocks, s);
-    return nch == 3 ? Launch<T, 4, 3, POST>::go(a, blocks, s) : Launch<T, 4, 4, POST>::go(a, blocks, s);
-}
-template <template <typename, int, int, bool> class Launch>
-static int rn_pick(int dtype, const RnArgs& a, int blocks, hipStream_t s) {
-    int wpr, nch;
-    rn_shape(a.cols, &wpr, &nch);
-    if (dtype == NEAT_F32)
-        return a.post_w ? rn_pick2<Launch, float, true>(wpr, nch, a, blocks, s) : rn_pick2<Launch, float, false>(wpr, nch, a, blocks, s);
-    return a.post_w ? rn_pick2<Launch, bf16_t, true>(wpr, nch, a, blocks, s) : rn_pick2<Launch, bf16_t, false>(wpr, nch, a, blocks, s);
-}
-template <typename T, int WPR, int NCH, bool POST> struct RnForward {
-    static int go(const RnArgs& a, int blocks, hipStream_t s) {
         hipLaunchKernelGGL((res_norm_fwd_kernel<T, WPR, NCH, POST>), dim3(blocks),
-                           dim3(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR), 0, s, a);
+                           dim3(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR), lds, s, a);
         NEAT_LAUNCH_CHECK("neat_res_norm_fwd");
         return NEAT_OK;
     }
+    static int pick(const RnArgs& a, int blocks, hipStream_t s) {
+        const int wpr = rn_fwd_wpr(a.cols);
+        switch (cdiv(a.cols / 4, 64 * wpr)) {
+            case 1: return go<1, 1>(a, blocks, s);
+            case 2: return go<1, 2>(a, blocks, s);
+            case 3: return go<1, 3>(a, blocks, s);
+            case 4: return go<1, 4>(a, blocks, s);
+            case 5: return wpr == 1 ? go<1, 5>(a, blocks, s) : go<2, 5>(a, blocks, s);
+            case 6: return wpr == 1 ? go<1, 6>(a, blocks, s) : go<2, 6>(a, blocks, s);
+            case 7: return wpr == 1 ? go<1, 7>(a, blocks, s) : go<2, 7>(a, blocks, s);
+            default: return wpr == 1 ? go<1, 8>(a, blocks, s) : go<2, 8>(a, blocks, s);
+        }
+    }
 };
-template <typename T, int WPR, int NCH, bool POST> struct RnBackward {
-    static int go(const RnArgs& a, int blocks, hipStream_t s) {
-        const size_t lds = WPR == 1 ? (size_t)RN_BWD_WAVES * a.cols * 4 : 0;
+template <typename T, bool POST> struct RnBackward {
+    template <int WPR, int NCH> static int go(const RnArgs& a, int blocks, hipStream_t s) {
+        const int teams = WPR == 1 ? RN_BWD_WAVES : 1, rows = 3 + (a.gate ? teams : 0);     // at least `teams`, for the sums
+        const size_t lds = (size_t)(rows > teams ? rows : teams) * a.cols * 4;
+        if (lds > RN_PLAIN_LDS) {
+            static unsigned long long done = 0;
+            if (int rc = ensure_dynamic_lds((const void*)res_norm_bwd_kernel<T, WPR, NCH, POST>, RN_MOST_LDS, &done, "neat_res_norm_bwd"))
+                return rc;
+        }
         hipLaunchKernelGGL((res_norm_bwd_kernel<T, WPR, NCH, POST>), dim3(blocks),
                            dim3(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR), lds, s, a);
         NEAT_LAUNCH_CHECK("neat_res_norm_bwd");
         return NEAT_OK;
     }
+    static int pick(const RnArgs& a, int blocks, hipStream_t s) {
+        const int wpr = rn_bwd_wpr(a.cols), nch = cdiv(a.cols / 4, 64 * wpr);
+        if (wpr == 1) {
+            switch (nch) {
+                case 1: return go<1, 1>(a, blocks, s);
+                case 2: return go<1, 2>(a, blocks, s);
+                case 3: return go<1, 3>(a, blocks, s);
+                default: return go<1, 4>(a, blocks, s);
+            }
+        }
+        if (wpr == 2) return nch == 3 ? go<2, 3>(a, blocks, s) : go<2, 4>(a, blocks, s);
+        return nch == 3 ? go<4, 3>(a, blocks, s) : go<4, 4>(a, blocks, s);
+    }
 };
+template <template <typename, bool> class Launch>
+static int rn_pick(int dtype, const RnArgs& a, int blocks, hipStream_t s) {
+    if (dtype == NEAT_F32) return a.post_w ? Launch<float, true>::pick(a, blocks, s) : Launch<float, false>::pick(a, blocks, s);
+    return a.post_w ? Launch<bf16_t, true>::pick(a, blocks, s) : Launch<bf16_t, false>::pick(a, blocks, s);
+}
 
 static bool rn_aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 static int rn_check(const char* who, const RnArgs& a, int dtype, int kind) {
@@ -496,13 +551,13 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     if (rows == 0) return NEAT_OK;
     NEAT_REQUIRE(x && h && pre_w && x_out && y, NEAT_ERR_ARG, "neat_res_norm_fwd: null pointer");
     const int blocks = rn_fwd_blocks(rows, cols);
-    a.teams = blocks * (cols <= 1024 ? RN_FWD_WAVES : 1);
+    a.teams = blocks * (rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1);
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
 }
 
 extern "C" long neat_res_norm_ws_floats(int rows, int cols, int groups) {
     if (rows < 0 || cols <= 0 || cols > RN_MAX_COLS || groups < 0) return 0;
-    const long blocks = rn_bwd_blocks(rows, cols), teams = blocks * (cols <= 1024 ? RN_BWD_WAVES : 1);
+    const long blocks = rn_bwd_blocks(rows, cols), teams = blocks * (rn_bwd_wpr(cols) == 1 ? RN_BWD_WAVES : 1);
     return blocks * RN_SUMS * cols + (groups ? (teams + groups) * cols : 0);
 }
 
@@ -521,7 +576,7 @@ extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* 
     NEAT_REQUIRE((!dpost_w && !dpost_b) || post_w, NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a norm that is not there");
     NEAT_REQUIRE((!dscale || scale) && (!dgate || gate), NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a scale or gate that is not there");
     const int blocks = rn_bwd_blocks(rows, cols);
-    a.teams = blocks * (cols <= 1024 ? RN_BWD_WAVES : 1);
+    a.teams = blocks * (rn_bwd_wpr(cols) == 1 ? RN_BWD_WAVES : 1);
     a.slots = gate ? ws + (long)blocks * RN_SUMS * cols : nullptr;
     hipStream_t s = (hipStream_t)stream;
     if (int rc = rn_pick<RnBackward>(dtype, a, blocks, s)) return rc;
