@@ -11,11 +11,10 @@
 //   N'(d) = r (z - mean z - uh mean(z uh)), z = d w (RMS: without mean z)
 //
 // Both directions read every input once and write every output once: 8 + 2t bytes an element forward, 12 + 3t backward (t = 2
-// for bf16, 4 for fp32).  A team of 1, 2 or 4 waves holds a row (up to 1 024 columns a wave, four 16-B chunks a lane) in
-// registers and takes a contiguous run of rows, balanced to one row whatever the groups' lengths.  Column sums stay in
-// registers over the run.  A group's sum is left behind at each group's end in slot team + group: runs and groups advance
-// together, so no two (team, group) pairs share a slot, and a second launch adds each group's slots, and the column sums, in
-// a fixed order: no atomics, equal bits on every run.
+// for bf16, 4 for fp32).  A team of 1 to 8 waves holds a row (up to five 16-B chunks a lane) in registers and takes a contiguous
+// run of rows, balanced to one row whatever the groups' lengths.  Column sums stay in registers over the run.  A group's sum is
+// left behind at each group's end in slot team + group: runs and groups advance together, so no two (team, group) pairs share a
+// slot, and a second launch adds each group's slots, and the column sums, in a fixed order: no atomics, equal bits on every run.
 #include "wave.h"
 
 namespace neat {
@@ -106,7 +105,7 @@ __device__ __forceinline__ int rn_group(const RnArgs& a, long row, long used) {
 // sums over a team; teams of several waves meet in LDS, two places in turn, so that one barrier a sum is enough
 template <int WPR>
 struct RnTeam {
-    float (*red)[2][4];
+    float (*red)[2][8];
     int turn;
     __device__ __forceinline__ void sum2(float& p, float& q) {
         p = row_sum(p);
@@ -180,10 +179,13 @@ __device__ __forceinline__ int rn_next_group(const RnArgs& a, int g, long row, l
     return g;
 }
 
+// waves a SIMD that the forward kernel's registers are kept to (wide: fp32 activations)
+constexpr int rn_fwd_waves(int nch, bool wide) { return nch == 1 ? 7 : nch == 2 ? 6 : nch <= 4 - wide ? 4 : 3; }
+
 template <typename T, int WPR, int NCH, bool POST>
-__global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR, NCH <= 2 ? 7 : NCH <= 4 ? 4 : NCH <= 6 ? 3 : 2) void res_norm_fwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR, rn_fwd_waves(NCH, sizeof(T) == 4)) void res_norm_fwd_kernel(RnArgs a) {
     constexpr int THREADS = WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR;
-    __shared__ float red[2][2][4];
+    __shared__ float red[2][2][8];
     extern __shared__ __attribute__((aligned(16))) f32x4 lds[];               // pre_w, pre_b, post_w, post_b: [4][cols]
     RnTeam<WPR> sums{red, 0};
     const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -258,9 +260,9 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR, NCH <= 2 ?
 // row and one wave more (14 851 x 768: 91 against 96 us in both directions).
 constexpr int rn_bwd_waves(int nch) { return nch == 1 ? 5 : nch == 2 ? 3 : 2; }
 template <typename T, int WPR, int NCH, bool POST>
-__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_waves(NCH)) void res_norm_bwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_waves(NCH) - (sizeof(T) == 4 && NCH == 1)) void res_norm_bwd_kernel(RnArgs a) {
     constexpr int TEAMS = WPR == 1 ? RN_BWD_WAVES : 1, THREADS = 64 * WPR * TEAMS;
-    __shared__ float red[2][2][4];
+    __shared__ float red[2][2][8];
     // pre_w, post_w, post_b: [3][cols]; behind them a team's sum of gate times group sums [TEAMS][cols]; at the end the sums
     extern __shared__ __attribute__((aligned(16))) f32x4 lds[];
     RnTeam<WPR> sums{red, 0};
@@ -307,11 +309,13 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_wav
 #pragma unroll
         for (int k = 0; k < 4; ++k) next.stat[k] = a.stats[(long)k * a.rows + row];
     };
-    if (run.lo < run.hi) fetch(run.lo);
+    constexpr bool AHEAD = sizeof(T) == 2 || NCH < 3;     // three chunks of fp32 leave no registers for a second row
+    if (AHEAD && run.lo < run.hi) fetch(run.lo);
     int g = -1;
     long end = a.gate ? run.lo : run.used;
     for (long row = run.lo; row < run.hi; ++row) {
         const long base = row * nch;
+        if (!AHEAD) fetch(row);
         f32x4 d[NCH], x[NCH], e[NCH], h[NCH];
         RN_EACH(i, c) {
             d[i] = RnIo<T>::open(next.d[i]);
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_wav
             h[i] = RnIo<T>::open(next.h[i]);
         }
         const float mu1 = next.stat[0], r1 = next.stat[1], mu2 = next.stat[2], r2 = next.stat[3];
-        if (row + 1 < run.hi) fetch(row + 1);             // the next row, while this one is worked on
+        if (AHEAD && row + 1 < run.hi) fetch(row + 1);    // the next row, while this one is worked on
         if (row >= end) {
             if (g >= 0) {
                 RN_EACH(i, c) {
@@ -466,19 +470,26 @@ __global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnAr
     if (g < a.groups && c < a.cols) o.gate[(long)g * a.cols + c] = a.scale ? s * a.scale[c] : s;
 }
 
-// waves of a team, and 16-B chunks a lane.  Forward a lane holds eight chunks of x and h without trouble; backward four, beside
-// five sums of them.
-static int rn_fwd_wpr(int cols) { return cols <= 2048 ? 1 : 2; }
-static int rn_bwd_wpr(int cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : 4; }
-static int rn_fwd_blocks(int rows, int cols) {
-    const int per = rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1;
-    const int b = cdiv(rows, per * 4), most = 8192 / per;
+// Waves of a team.  Forward a lane holds up to five chunks of x and h, backward three beside five sums of them: with four the
+// registers spill (30 M elements backward, TB/s with four / three chunks: 1 024 columns 1.8 / 4.7, 2 048 1.6 / 4.9).
+constexpr int RN_BWD_COLS = 768;                          // of one wave backward: three chunks a lane
+static int rn_fwd_wpr(int cols) { return cols <= 1280 ? 1 : 4; }
+static int rn_bwd_wpr(int cols) { return cols <= RN_BWD_COLS ? 1 : cols <= 2 * RN_BWD_COLS ? 2 : cols <= 4 * RN_BWD_COLS ? 4 : 8; }
+// As many workgroups as fit the chip's 256 CUs at once, by registers and LDS (forward every workgroup has four waves), and four
+// rows a team where there are that many.  One round of workgroups that all run: 30 M elements forward at 256 / 1 664 / 2 560 /
+// 4 096 columns 4.8 / 4.4 / 4.2 / 3.3 TB/s with 8 192 teams whatever fits, 5.6 / 5.6 / 5.4 / 5.3 so.
+static int rn_fwd_blocks(int rows, int cols, bool wide) {
+    const int wpr = rn_fwd_wpr(cols), per = wpr == 1 ? RN_FWD_WAVES : 1;
+    const int waves = rn_fwd_waves(cdiv(cols / 4, 64 * wpr), wide), by_lds = 160 * 1024 / (16 * cols + 64);
+    const int most = 256 * (by_lds < waves ? by_lds : waves);
+    const int all = cdiv(rows, per), few = all < 256 ? all : 256;
+    int b = cdiv(rows, per * 4);
+    b = b < few ? few : b;
     return b < 1 ? 1 : b > most ? most : b;
 }
 static int rn_bwd_blocks(int rows, int cols) {
-    // as many as fit the chip at once (256 CUs, 4 SIMDs each): more would leave more partial sums behind, and fewer fill less
-    const int wpr = rn_bwd_wpr(cols), per = wpr == 1 ? RN_BWD_WAVES : 1, nch = cdiv(cols / 4, 64 * wpr);
-    const int most = 256 * 4 * rn_bwd_waves(nch) / (wpr * per);
+    const int wpr = rn_bwd_wpr(cols), per = wpr == 1 ? RN_BWD_WAVES : 1;
+    const int most = 256 * 4 * rn_bwd_waves(cdiv(cols / 4, 64 * wpr)) / (wpr * per);
     const int b = cdiv(rows, per * 2);
     return b < 1 ? 1 : b > most ? most : b;
 }
@@ -501,16 +512,17 @@ template <typename T, bool POST> struct RnForward {
     }
     static int pick(const RnArgs& a, int blocks, hipStream_t s) {
         const int wpr = rn_fwd_wpr(a.cols);
-        switch (cdiv(a.cols / 4, 64 * wpr)) {
-            case 1: return go<1, 1>(a, blocks, s);
-            case 2: return go<1, 2>(a, blocks, s);
-            case 3: return go<1, 3>(a, blocks, s);
-            case 4: return go<1, 4>(a, blocks, s);
-            case 5: return wpr == 1 ? go<1, 5>(a, blocks, s) : go<2, 5>(a, blocks, s);
-            case 6: return wpr == 1 ? go<1, 6>(a, blocks, s) : go<2, 6>(a, blocks, s);
-            case 7: return wpr == 1 ? go<1, 7>(a, blocks, s) : go<2, 7>(a, blocks, s);
-            default: return wpr == 1 ? go<1, 8>(a, blocks, s) : go<2, 8>(a, blocks, s);
+        const int nch = cdiv(a.cols / 4, 64 * wpr);
+        if (wpr == 1) {
+            switch (nch) {
+                case 1: return go<1, 1>(a, blocks, s);
+                case 2: return go<1, 2>(a, blocks, s);
+                case 3: return go<1, 3>(a, blocks, s);
+                case 4: return go<1, 4>(a, blocks, s);
+                default: return go<1, 5>(a, blocks, s);
+            }
         }
+        return nch == 2 ? go<4, 2>(a, blocks, s) : nch == 3 ? go<4, 3>(a, blocks, s) : go<4, 4>(a, blocks, s);
     }
 };
 template <typename T, bool POST> struct RnBackward {
@@ -529,16 +541,10 @@ template <typename T, bool POST> struct RnBackward {
     }
     static int pick(const RnArgs& a, int blocks, hipStream_t s) {
         const int wpr = rn_bwd_wpr(a.cols), nch = cdiv(a.cols / 4, 64 * wpr);
-        if (wpr == 1) {
-            switch (nch) {
-                case 1: return go<1, 1>(a, blocks, s);
-                case 2: return go<1, 2>(a, blocks, s);
-                case 3: return go<1, 3>(a, blocks, s);
-                default: return go<1, 4>(a, blocks, s);
-            }
-        }
-        if (wpr == 2) return nch == 3 ? go<2, 3>(a, blocks, s) : go<2, 4>(a, blocks, s);
-        return nch == 3 ? go<4, 3>(a, blocks, s) : go<4, 4>(a, blocks, s);
+        if (wpr == 1) return nch == 1 ? go<1, 1>(a, blocks, s) : nch == 2 ? go<1, 2>(a, blocks, s) : go<1, 3>(a, blocks, s);
+        if (wpr == 2) return nch == 2 ? go<2, 2>(a, blocks, s) : go<2, 3>(a, blocks, s);
+        if (wpr == 4) return nch == 2 ? go<4, 2>(a, blocks, s) : go<4, 3>(a, blocks, s);
+        return go<8, 2>(a, blocks, s);
     }
 };
 template <template <typename, bool> class Launch>
@@ -582,7 +588,7 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     if (int rc = rn_check("neat_res_norm_fwd", a, dtype, kind)) return rc;
     if (rows == 0) return NEAT_OK;
     NEAT_REQUIRE(x && h && pre_w && x_out && y, NEAT_ERR_ARG, "neat_res_norm_fwd: null pointer");
-    const int blocks = rn_fwd_blocks(rows, cols);
+    const int blocks = rn_fwd_blocks(rows, cols, dtype == NEAT_F32);
     a.teams = blocks * (rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1);
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
 }
