@@ -86,7 +86,7 @@ int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const 
  * (gradient of x) and dh (of dtype), and the sums over rows dpre_w .. dscale f32 [cols], dgate f32 [groups, cols] (NULL: not
  * wanted; written, not added to).  stats, x_out from the forward pass.  ws: neat_res_norm_ws_floats floats, 16-byte aligned.
  * Sums are formed in a fixed order. */
-long neat_res_norm_ws_floats(int rows, int cols, int groups);
+long neat_res_norm_ws_floats(int dtype, int rows, int cols, int groups);
 int neat_res_norm_bwd(const void* dy, const float* dres, const void* h, const float* x_out, const float* stats, int dtype, int kind,
                       const float* pre_w, const float* post_w, const float* post_b, const float* scale, const float* gate,
                       int groups, const int32_t* cu, float* dx, void* dh, float* dpre_w, float* dpre_b, float* dpost_w,

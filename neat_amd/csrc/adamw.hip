@@ -22,6 +22,7 @@ namespace neat {
 constexpr int AW_BLOCK = 256;       // elements per block of moments = 16 lanes x 16
 constexpr int AW_WAVES = 4;
 constexpr int AW_UNIT = 4;          // blocks a wave takes, one for each row of 16 lanes
+constexpr long AW_MOST = 1L << 26;   // units of a launch: 2^32 work items are the limit
 constexpr int AW_TENSORS = 96;      // 96 x 40 B of kernel arguments beside the launch's own ~80 B; 4 096 B is the limit
 
 struct AwTensor {
@@ -187,6 +188,7 @@ __device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f
                                         const AwTensor& t) {
     f32x4 m[4], v[4], r[4];
     uint32_t zeros = 0;
+    bool odd = false;                                   // a moment that is subnormal or infinite
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if constexpr (SMALL) {
@@ -208,8 +210,28 @@ __device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f
             m[k][j] = m[k][j] + (g[k][j] - m[k][j]) * a.omb1;
             v[k][j] = v[k][j] * a.b2 + g[k][j] * g[k][j] * a.omb2;
             // root and reciprocal of the hardware (one unit in the last place each): the step they scale is added to a
-            // parameter that is larger by orders of magnitude
-            r[k][j] = __builtin_amdgcn_sqrtf(v[k][j]);
+            // parameter that is larger by orders of magnitude.  A root that is held in 8 bits is corrected once, so that next to
+            // no code is another than the exact root's
+            if constexpr (SMALL) {
+                const float y = __builtin_amdgcn_rsqf(fmaxf(v[k][j], 0x1p-126f)), x = v[k][j] * y;
+                r[k][j] = __builtin_fmaf(__builtin_fmaf(-x, x, v[k][j]), 0.5f * y, x);
+            } else {
+                r[k][j] = __builtin_amdgcn_sqrtf(v[k][j]);
+            }
+            odd |= __builtin_amdgcn_classf(v[k][j], 0x280);
+        }
+    }
+    if (__any(odd)) {                                   // the hardware's root takes a subnormal for zero
+        asm volatile("");
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[k][j] = sqrtf(v[k][j]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             const float u = m[k][j] * __builtin_amdgcn_rcpf(__builtin_fmaf(r[k][j], t.inv_sqrt_bc2, a.eps));
             p[k][j] = __builtin_fmaf(-t.step_size, u, p[k][j] * a.decay);
         }
@@ -352,7 +374,7 @@ extern "C" int neat_adamw_multi(int count, void* const* p, const void* const* g,
     for (int i = 0; i < count; ++i) {                   // everything is checked before anything is launched
         NEAT_REQUIRE(n[i] >= 0 && state_block[i] >= 0, NEAT_ERR_SHAPE, "neat_adamw_multi: tensor %d: n=%ld state_block=%ld", i,
                      (long)n[i], (long)state_block[i]);
-        NEAT_REQUIRE(n[i] < (1L << 38) && state_block[i] < (1L << 32) - (1L << 30), NEAT_ERR_SHAPE,
+        NEAT_REQUIRE(n[i] < AW_MOST * AW_UNIT * AW_BLOCK && state_block[i] < (1L << 32) - AW_MOST * AW_UNIT, NEAT_ERR_SHAPE,
                      "neat_adamw_multi: tensor %d too large", i);
         NEAT_REQUIRE(step[i] >= 1, NEAT_ERR_SHAPE, "neat_adamw_multi: tensor %d: step=%d", i, step[i]);
         NEAT_REQUIRE(n[i] == 0 || (p[i] && g[i]), NEAT_ERR_ARG, "neat_adamw_multi: tensor %d: null pointer", i);
@@ -375,7 +397,7 @@ extern "C" int neat_adamw_multi(int count, void* const* p, const void* const* g,
         for (; i < count && a.count < AW_TENSORS; ++i) {
             if (n[i] == 0) continue;
             const long nu = (n[i] + AW_BLOCK * AW_UNIT - 1) / (AW_BLOCK * AW_UNIT);
-            if (units + nu > (1L << 31)) break;
+            if (units + nu > AW_MOST) break;           // one tensor alone always fits
             if (step[i] != known) {                     // mostly one step count for all: two pow per launch
                 known = step[i];
                 step_size = (float)(lr / (1.0 - pow(beta1, known)));

@@ -309,13 +309,11 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_wav
 #pragma unroll
         for (int k = 0; k < 4; ++k) next.stat[k] = a.stats[(long)k * a.rows + row];
     };
-    constexpr bool AHEAD = sizeof(T) == 2 || NCH < 3;     // three chunks of fp32 leave no registers for a second row
-    if (AHEAD && run.lo < run.hi) fetch(run.lo);
+    if (run.lo < run.hi) fetch(run.lo);
     int g = -1;
     long end = a.gate ? run.lo : run.used;
     for (long row = run.lo; row < run.hi; ++row) {
         const long base = row * nch;
-        if (!AHEAD) fetch(row);
         f32x4 d[NCH], x[NCH], e[NCH], h[NCH];
         RN_EACH(i, c) {
             d[i] = RnIo<T>::open(next.d[i]);
@@ -324,7 +322,7 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_wav
             h[i] = RnIo<T>::open(next.h[i]);
         }
         const float mu1 = next.stat[0], r1 = next.stat[1], mu2 = next.stat[2], r2 = next.stat[3];
-        if (AHEAD && row + 1 < run.hi) fetch(row + 1);    // the next row, while this one is worked on
+        if (row + 1 < run.hi) fetch(row + 1);             // the next row, while this one is worked on
         if (row >= end) {
             if (g >= 0) {
                 RN_EACH(i, c) {
@@ -472,9 +470,13 @@ __global__ __launch_bounds__(64 * RNF_SLICES) void res_norm_finalize_kernel(RnAr
 
 // Waves of a team.  Forward a lane holds up to five chunks of x and h, backward three beside five sums of them: with four the
 // registers spill (30 M elements backward, TB/s with four / three chunks: 1 024 columns 1.8 / 4.7, 2 048 1.6 / 4.9).
-constexpr int RN_BWD_COLS = 768;                          // of one wave backward: three chunks a lane
+// fp32 activations take twice the registers in flight: two chunks (20 M elements backward at 768 columns 3.9 TB/s with three).
+static int rn_bwd_wave_cols(bool wide) { return wide ? 512 : 768; }
 static int rn_fwd_wpr(int cols) { return cols <= 1280 ? 1 : 4; }
-static int rn_bwd_wpr(int cols) { return cols <= RN_BWD_COLS ? 1 : cols <= 2 * RN_BWD_COLS ? 2 : cols <= 4 * RN_BWD_COLS ? 4 : 8; }
+static int rn_bwd_wpr(int cols, bool wide) {
+    const int w = rn_bwd_wave_cols(wide);
+    return cols <= w ? 1 : cols <= 2 * w ? 2 : cols <= 4 * w ? 4 : 8;
+}
 // As many workgroups as fit the chip's 256 CUs at once, by registers and LDS (forward every workgroup has four waves), and four
 // rows a team where there are that many.  One round of workgroups that all run: 30 M elements forward at 256 / 1 664 / 2 560 /
 // 4 096 columns 4.8 / 4.4 / 4.2 / 3.3 TB/s with 8 192 teams whatever fits, 5.6 / 5.6 / 5.4 / 5.3 so.
@@ -487,8 +489,8 @@ static int rn_fwd_blocks(int rows, int cols, bool wide) {
     b = b < few ? few : b;
     return b < 1 ? 1 : b > most ? most : b;
 }
-static int rn_bwd_blocks(int rows, int cols) {
-    const int wpr = rn_bwd_wpr(cols), per = wpr == 1 ? RN_BWD_WAVES : 1;
+static int rn_bwd_blocks(int rows, int cols, bool wide) {
+    const int wpr = rn_bwd_wpr(cols, wide), per = wpr == 1 ? RN_BWD_WAVES : 1;
     const int most = 256 * 4 * rn_bwd_waves(cdiv(cols / 4, 64 * wpr)) / (wpr * per);
     const int b = cdiv(rows, per * 2);
     return b < 1 ? 1 : b > most ? most : b;
@@ -540,11 +542,12 @@ template <typename T, bool POST> struct RnBackward {
         return NEAT_OK;
     }
     static int pick(const RnArgs& a, int blocks, hipStream_t s) {
-        const int wpr = rn_bwd_wpr(a.cols), nch = cdiv(a.cols / 4, 64 * wpr);
-        if (wpr == 1) return nch == 1 ? go<1, 1>(a, blocks, s) : nch == 2 ? go<1, 2>(a, blocks, s) : go<1, 3>(a, blocks, s);
-        if (wpr == 2) return nch == 2 ? go<2, 2>(a, blocks, s) : go<2, 3>(a, blocks, s);
-        if (wpr == 4) return nch == 2 ? go<4, 2>(a, blocks, s) : go<4, 3>(a, blocks, s);
-        return go<8, 2>(a, blocks, s);
+        const int wpr = rn_bwd_wpr(a.cols, sizeof(T) == 4), nch = cdiv(a.cols / 4, 64 * wpr);
+        if constexpr (sizeof(T) == 2) {
+            if (nch == 3) return wpr == 1 ? go<1, 3>(a, blocks, s) : wpr == 2 ? go<2, 3>(a, blocks, s) : go<4, 3>(a, blocks, s);
+        }
+        if (nch == 1) return go<1, 1>(a, blocks, s);
+        return wpr == 1 ? go<1, 2>(a, blocks, s) : wpr == 2 ? go<2, 2>(a, blocks, s) : wpr == 4 ? go<4, 2>(a, blocks, s) : go<8, 2>(a, blocks, s);
     }
 };
 template <template <typename, bool> class Launch>
@@ -593,9 +596,10 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
 }
 
-extern "C" long neat_res_norm_ws_floats(int rows, int cols, int groups) {
+extern "C" long neat_res_norm_ws_floats(int dtype, int rows, int cols, int groups) {
     if (rows < 0 || cols <= 0 || cols > RN_MAX_COLS || groups < 0) return 0;
-    const long blocks = rn_bwd_blocks(rows, cols), teams = blocks * (rn_bwd_wpr(cols) == 1 ? RN_BWD_WAVES : 1);
+    const bool wide = dtype == NEAT_F32;
+    const long blocks = rn_bwd_blocks(rows, cols, wide), teams = blocks * (rn_bwd_wpr(cols, wide) == 1 ? RN_BWD_WAVES : 1);
     return blocks * RN_SUMS * cols + (groups ? (teams + groups) * cols : 0);
 }
 
@@ -613,8 +617,9 @@ extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* 
     NEAT_REQUIRE(pre_w && ws, NEAT_ERR_ARG, "neat_res_norm_bwd: null pointer");
     NEAT_REQUIRE((!dpost_w && !dpost_b) || post_w, NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a norm that is not there");
     NEAT_REQUIRE((!dscale || scale) && (!dgate || gate), NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a scale or gate that is not there");
-    const int blocks = rn_bwd_blocks(rows, cols);
-    a.teams = blocks * (rn_bwd_wpr(cols) == 1 ? RN_BWD_WAVES : 1);
+    const bool wide = dtype == NEAT_F32;
+    const int blocks = rn_bwd_blocks(rows, cols, wide);
+    a.teams = blocks * (rn_bwd_wpr(cols, wide) == 1 ? RN_BWD_WAVES : 1);
     a.slots = gate ? ws + (long)blocks * RN_SUMS * cols : nullptr;
     hipStream_t s = (hipStream_t)stream;
     if (int rc = rn_pick<RnBackward>(dtype, a, blocks, s)) return rc;

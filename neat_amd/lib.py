@@ -27,7 +27,7 @@ SIGNATURES = {
     "neat_ln_bwd_finalize": (_I, [_P, _I, _I, _P, _P, _I, _P]),
     "neat_ln_bwd_finalize_batched": (_I, [_P, _I, _I, _I, _P, _I, _P]),
     "neat_res_norm_fwd": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
-    "neat_res_norm_ws_floats": (_L, [_I, _I, _I]),
+    "neat_res_norm_ws_floats": (_L, [_I, _I, _I, _I]),
     "neat_res_norm_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I,
                                _P]),
     "neat_pack_weight_bf16": (_I, [_P, _P, _I, _I, _I, _P]),

@@ -182,36 +182,49 @@ _NORMS = {"ln": lib.NORM_LAYER, "rms": lib.NORM_RMS}
 
 
 def _res_norm_args(who, x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu, kind):
-    """Checks what both directions share -> (rows, cols, groups, dtype, kind, device)."""
+    """Checks what both directions share -> (rows, cols, groups, dtype, kind, device index, the pointers of x, h and the
+    parameters).  Written for small calls: a token's junction takes the GPU less time than a careless check of ten tensors."""
     if kind not in _NORMS:
         raise RuntimeError(f"{who}: kind must be 'ln' or 'rms', got {kind!r}")
-    if x.dim() != 2 or h.shape != x.shape or h.dtype not in _DTYPES:
-        raise RuntimeError(f"{who}: expected [rows, cols], float32 stream and float32 or bfloat16 branch, got "
-                           f"{tuple(x.shape)} and {h.dtype} {tuple(h.shape)}")
+    dt = _DTYPES.get(h.dtype)
+    if x.dim() != 2 or h.shape != x.shape or dt is None or x.dtype != f32:
+        raise RuntimeError(f"{who}: expected [rows, cols], float32 stream and float32 or bfloat16 branch; got the dtypes "
+                           f"{x.dtype}, {h.dtype} and shapes {tuple(x.shape)}, {tuple(h.shape)}")
     rows, cols = x.shape
+    index = x.get_device()
+    if index < 0:
+        raise RuntimeError(f"{who}: expected GPU tensors (libneat_hip has no CPU path)")
+    if not (x.is_contiguous() and h.is_contiguous() and h.get_device() == index):
+        raise RuntimeError(f"{who}: stream and branch must be contiguous, on one device")
+    ptrs = [x.data_ptr(), h.data_ptr()]
     for t, nm in ((pre_w, "pre_w"), (pre_b, "pre_b"), (post_w, "post_w"), (post_b, "post_b"), (scale, "scale")):
-        if t is not None and (tuple(t.shape) != (cols,) or t.device != x.device):
-            raise RuntimeError(f"{who}: {nm} must be float32 [{cols}] on the stream's device")
+        if t is None:
+            ptrs.append(None)
+        elif t.dim() != 1 or t.numel() != cols or t.dtype != f32 or not t.is_contiguous() or t.get_device() != index:
+            raise RuntimeError(f"{who}: {nm} must be contiguous float32 [{cols}] on the stream's device")
+        else:
+            ptrs.append(t.data_ptr())
     if post_b is not None and post_w is None:
         raise RuntimeError(f"{who}: post_b without post_w")
     groups = 0
     if gate is not None:
         groups = gate.shape[0]
-        if gate.dim() != 2 or gate.shape[1] != cols or groups < 1 or gate.device != x.device:
+        if gate.dim() != 2 or gate.shape[1] != cols or groups < 1 or gate.get_device() != index:
             raise RuntimeError(f"{who}: gate must be float32 [groups, {cols}] on the stream's device")
         if cu is None and rows % groups:
             raise RuntimeError(f"{who}: {rows} rows do not divide into {groups} groups (pass cu)")
-    if cu is not None and (gate is None or tuple(cu.shape) != (groups + 1,) or cu.device != x.device):
+    if cu is not None and (gate is None or tuple(cu.shape) != (groups + 1,) or cu.get_device() != index):
         raise RuntimeError(f"{who}: cu must be int32 [groups + 1] beside a gate")
-    return rows, cols, groups, _DTYPES[h.dtype], _NORMS[kind], x.device
+    ptrs += [_p(gate, f32, "gate"), groups, _p(cu, i32, "cu")]
+    return rows, cols, groups, dt, _NORMS[kind], x.device, ptrs
 
 
 def _res_norm_out(t, like, dtype, who):
     """(tensor, whether rows behind the last group are to be zeroed: in a buffer made here they hold nothing)."""
     if t is None:
-        return torch.empty(like.shape, dtype=dtype, device=like.device), True
-    if t.shape != like.shape or t.device != like.device:
-        raise RuntimeError(f"{who}: an output has another shape or device than its input")
+        return torch.empty_like(like, dtype=dtype), True
+    if t.shape != like.shape or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
+        raise RuntimeError(f"{who}: an output must be contiguous {dtype} {tuple(like.shape)} on its input's device")
     return t, False
 
 
@@ -223,20 +236,19 @@ def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, 
     x_out = x + N_post(h) * scale * gate, y = N_pre(x_out) -> (x_out, y in h's type, stats for ``res_norm_bwd`` or None).
     ``kind``: "ln" or "rms".  Groups are rows // groups rows each, or the sequences of a packed batch (``cu`` int32 [groups
     + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (x_out may be x), zero in new ones."""
-    rows, cols, groups, dt, kd, dev = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu, kind)
+    rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu,
+                                                           kind)
     x_out, zx = _res_norm_out(x_out, x, f32, "res_norm_fwd")
     y, zy = _res_norm_out(y, h, h.dtype, "res_norm_fwd")
     stats = torch.empty(4, rows, dtype=f32, device=dev) if save else None
-    _call_on(dev, "neat_res_norm_fwd", _p(x, f32, "x"), _p(h, None, "h"), dt, kd, _p(pre_w, f32, "pre_w"), _p(pre_b, f32, "pre_b"),
-             _p(post_w, f32, "post_w"), _p(post_b, f32, "post_b"), _p(scale, f32, "scale"), _p(gate, f32, "gate"), groups,
-             _p(cu, i32, "cu"), _p(x_out, f32, "x_out"), _p(y, h.dtype, "y"), _ptr(stats),
-             (int(zx) | 2 * int(zy)) if cu is not None else 0, rows, cols, float(eps))
+    _call_on(dev, "neat_res_norm_fwd", ptrs[0], ptrs[1], dt, kd, *ptrs[2:], x_out.data_ptr(), y.data_ptr(), _ptr(stats),
+             (int(zx) | 2 * int(zy)) if cu is not None else 0, rows, cols, eps)
     return x_out, y, stats
 
 
 @functools.lru_cache(maxsize=256)
-def _res_norm_ws_floats(rows, cols, groups):
-    return lib.load().neat_res_norm_ws_floats(rows, cols, groups)
+def _res_norm_ws_floats(dt, rows, cols, groups):
+    return lib.load().neat_res_norm_ws_floats(dt, rows, cols, groups)
 
 
 def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, scale=None, gate=None, cu=None, kind="ln", dx=None,
@@ -244,7 +256,8 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
     """Backward of ``res_norm_fwd``: dy = gradient of y (h's type), dres = gradient of x_out from elsewhere (float32 or None) ->
     (dx float32, dh in h's type, {"pre_w", "pre_b", "post_w", "post_b", "scale", "gate"}: float32 gradients of what was given;
     those of a bias are there with their weight's).  ``dx`` may be dres.  Sums are formed in a fixed order."""
-    rows, cols, groups, dt, kd, dev = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu, kind)
+    rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu,
+                                                           kind)
     if dy.shape != h.shape or dy.device != dev or tuple(stats.shape) != (4, rows) or stats.device != dev:
         raise RuntimeError("res_norm_bwd: dy must have the branch's shape and stats be the forward pass's [4, rows]")
     if dres is not None and (dres.shape != x_out.shape or dres.device != dev):
@@ -254,13 +267,13 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
     names = ["pre_w", "pre_b"] + (["post_w", "post_b"] if post_w is not None else []) + (["scale"] if scale is not None else [])
     grads = dict(zip(names, torch.empty(len(names), cols, dtype=f32, device=dev).unbind(0)))
     if gate is not None:
-        grads["gate"] = torch.empty(groups, cols, dtype=f32, device=dev)
-    ws = torch.empty(_res_norm_ws_floats(rows, cols, groups), dtype=f32, device=dev)
+        grads["gate"] = torch.empty_like(gate)
+    ws = torch.empty(_res_norm_ws_floats(dt, rows, cols, groups), dtype=f32, device=dev)
     g = [_ptr(grads.get(n)) for n in ("pre_w", "pre_b", "post_w", "post_b", "scale", "gate")]
-    _call_on(dev, "neat_res_norm_bwd", _p(dy, h.dtype, "dy"), _p(dres, f32, "dres"), _p(h, None, "h"), _p(x_out, f32, "x_out"),
-             _p(stats, f32, "stats"), dt, kd, _p(pre_w, f32, "pre_w"), _p(post_w, f32, "post_w"), _p(post_b, f32, "post_b"),
-             _p(scale, f32, "scale"), _p(gate, f32, "gate"), groups, _p(cu, i32, "cu"), _p(dx, f32, "dx"), _p(dh, h.dtype, "dh"),
-             *g, ws.data_ptr(), (int(zx) | 2 * int(zh)) if cu is not None else 0, rows, cols)
+    xp, hp, wp, _, pw, pb, sc, gp, _, cp = ptrs
+    _call_on(dev, "neat_res_norm_bwd", _p(dy, h.dtype, "dy"), _p(dres, f32, "dres"), hp, xp, _p(stats, f32, "stats"), dt, kd, wp, pw,
+             pb, sc, gp, groups, cp, dx.data_ptr(), dh.data_ptr(), *g, ws.data_ptr(),
+             (int(zx) | 2 * int(zh)) if cu is not None else 0, rows, cols)
     return dx, dh, grads
 
 

@@ -266,3 +266,36 @@ def test_transposed_gradient_empty_tensor_and_refusals():
         ops.adamw_multi([w], [w.grad.contiguous()], [1], [1], m, torch.zeros_like(m))
     with pytest.raises(RuntimeError, match="step=0"):
         ops.adamw_multi([w], [w.grad.contiguous()], [0], [0], m, torch.zeros_like(m))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("g", [1e-10, 1e-18, 1e-19, 1e-20])
+def test_gradients_whose_square_is_subnormal(bits, g):
+    """The second moment (1e-3 g^2) is a subnormal float32 here, which holds it to 2^-149: off by at most 2^-150 / (1e-3 g^2) of
+    itself, the step by half of that.  It stays above zero, and the step is no larger than with any other gradient."""
+    p = torch.nn.Parameter(torch.zeros(300, device=DEV))
+    p.grad = torch.full_like(p, g)
+    p.grad[::7] = 0.0
+    opt = MultiTensorAdamW([p], lr=LR, betas=(B1, B2), eps=1e-30, weight_decay=0.0, state_bits=bits)
+    opt.step()
+    m, v, _ = opt.moments(p)
+    some = p.grad > 0
+    rel = 16 * U + 0.5 * 2.0 ** -150 / (1e-3 * g * g) * 1.01
+    assert ((p.detach().double() / -LR - 1).abs()[some] <= rel + g * 0).all() and (p[~some] == 0).all()
+    if bits == 32:
+        assert ((v > 0) == some).all()
+    else:
+        assert ((opt.exp_avg_root.float().view(-1)[:300] > 0) == some).all()
+
+
+def test_a_scalar_parameter_and_a_closure():
+    p = torch.nn.Parameter(torch.tensor(2.0, device=DEV))
+    opt = MultiTensorAdamW([p], lr=LR, weight_decay=0.0)
+
+    def closure():
+        opt.zero_grad()
+        loss = 3.0 * p
+        loss.backward()
+        return loss
+    assert float(opt.step(closure)) == 6.0
+    assert abs(float(p) - (2.0 - LR)) <= 4 * U and opt.moments(p)[0].shape == ()

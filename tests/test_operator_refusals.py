@@ -128,5 +128,5 @@ def test_res_norm_backward_checks_before_launching():
     for bad in (dict(dy=None), dict(stats=None), dict(ws=None), dict(post_w=None), dict(scale=None), dict(gate=None, groups=0),
                 dict(ws=72)):
         assert call(**bad) == -2, bad
-    assert L.neat_res_norm_ws_floats(4, 64, 2) > 5 * 64
+    assert L.neat_res_norm_ws_floats(0, 4, 64, 2) > 5 * 64
     assert _rn(rows=0) == 0
