@@ -144,7 +144,6 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise RuntimeError("MultiTensorAdamW: the moments are laid out when it is built; pass all groups then")
         super().add_param_group(group)
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
