@@ -68,8 +68,8 @@ int neat_ln_bwd_finalize(const float* partial, int nblk, int cols, float* dgamma
 int neat_ln_bwd_finalize_batched(const float* partial, int nblk, int cols, int count, float* const* dst,
                                  int accumulate, void* stream);
 
-/* ---- the norms around a block with its gate and residual scale (LayerScale, open_clip/transformer.py:46-53, :234-243; norms
- * behind the branches, :246-289) ---- */
+/* ---- the norms around a block with its gate and residual scale (towers with LayerScale, with norms behind their blocks, or
+ * with gates per sequence; a plain block's junction is open_clip/transformer.py:241-242) ---- */
 /* n = N_post(h) (post_w NULL: h); x_out = x + n * scale[c] * gate[g, c]; y = N_pre(x_out).  kind: NEAT_NORM_LAYER (mean taken
  * off, biased variance) or NEAT_NORM_RMS, both norms alike, eps inside the root.  x, x_out f32 [rows, cols] (x_out may be x);
  * h, y of `dtype` (NEAT_F32 / NEAT_BF16); weights, scale f32 [cols], gate f32 [groups, cols]; pre_b, post_w, post_b, scale,

@@ -11,8 +11,11 @@
 // beside a first moment that is not would blow the next step up.  The step itself uses the moments before they are rounded.
 //
 // Mapping: a wave takes four blocks, a row of 16 lanes each, four times four contiguous elements a lane: whole 256-B runs of
-// fp32 per row and load, one reduction for four blocks, and all loads of a unit in flight together.  Tensor addresses travel as kernel arguments (96 tensors a launch): no table in device memory, so no copy to order
-// behind other work and none to keep alive.
+// fp32 per row and load, one reduction for four blocks, and all loads of a unit in flight together.  Tensor addresses travel as
+// kernel arguments (96 tensors a launch): no table in device memory, so no copy to order behind other work and none to keep alive.
+//
+// Bound by HBM: 37.7 M fp32 parameters in 144 tensors 187 us (1 059 MB, 5.7 TB/s); in bf16 with 8-bit moments 82 us (381 MB, 4.6
+// TB/s, and about what the host needs to pass 144 tensors).  Small tensors are bound by the host: 6 us of 31 for 48 x 512.
 #include <math.h>
 
 #include "common.h"
@@ -22,7 +25,7 @@ namespace neat {
 constexpr int AW_BLOCK = 256;       // elements per block of moments = 16 lanes x 16
 constexpr int AW_WAVES = 4;
 constexpr int AW_UNIT = 4;          // blocks a wave takes, one for each row of 16 lanes
-constexpr long AW_MOST = 1L << 26;   // units of a launch: 2^32 work items are the limit
+constexpr long AW_MOST = 1L << 26;  // units of a launch: 2^32 work items are the limit
 constexpr int AW_TENSORS = 96;      // 96 x 40 B of kernel arguments beside the launch's own ~80 B; 4 096 B is the limit
 
 struct AwTensor {
@@ -44,9 +47,9 @@ struct AwLaunch {
 };
 static_assert(sizeof(AwLaunch) <= 4096, "kernel arguments");
 
-// Everything is touched once a step: loaded and stored past the caches (37.7 M fp32 parameters 210 -> 191 us, 5.5 TB/s).
-// Gradients are often views of a communication bucket that start at any element: loads of four elements need the element's own
-// alignment only (global memory takes unaligned wide accesses)
+// Everything is touched once a step: loaded and stored past the caches (37.7 M fp32 parameters 210 -> 191 us).  Gradients are
+// often views of a communication bucket that start at any element: loads of four elements need the element's own alignment
+// only (global memory takes unaligned wide accesses).
 template <typename T> struct AwIo;
 template <> struct AwIo<float> {
     typedef float vec __attribute__((ext_vector_type(4), aligned(4)));

@@ -14,6 +14,11 @@
 // collected and ranked by counting (value, then lower index): no sort, and no atomic that matters to the result.  Where many
 // reach it (a row of few different values, or mostly masked), 64-bit keys (value, index) that never tie take its place: the
 // k-th largest of up to 256 groups' keys leaves at most k groups' elements, for which there is room.
+//
+// Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 186 us (974 MB, 5.2 TB/s), 2 000 x 25 014 fp32
+// with 10 alternatives 45 us (200 MB, 4.4 TB/s; the ranking of one row runs under the loads of another).  One row of 49 408 with
+// 5 alternatives: 10 us, half of it the exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining
+// launch takes 1 us with them, so rows are cut only where they do not fit.
 #include "wave.h"
 
 namespace neat {
