@@ -89,16 +89,18 @@ __device__ __forceinline__ void lp_store(T* p, long i, u32x4 v) {
     __builtin_nontemporal_store((typename LpIo<T>::vec)v, reinterpret_cast<typename LpIo<T>::vec*>(p + i));
 }
 
-// value order as an unsigned number, -0 as +0, NaN as -inf; the smaller index is the larger key.  No element's key is 0.
-__device__ __forceinline__ uint64_t lp_key(float x, uint32_t i) {
+// value order as an unsigned number, -0 as +0, NaN as -inf
+__device__ __forceinline__ uint32_t lp_order(float x) {
     x = x == x ? x + 0.f : -INFINITY;
     const uint32_t u = __float_as_uint(x);
-    return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - i);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float lp_value(uint64_t key) {
-    const uint32_t u = (uint32_t)(key >> 32);
+__device__ __forceinline__ float lp_from_order(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
+// an element's key: value, then the smaller index as the larger one.  No element's key is 0.
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t i) { return (uint64_t)lp_order(x) << 32 | (0xffffffffu - i); }
+__device__ __forceinline__ float lp_value(uint64_t key) { return lp_from_order((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int32_t lp_index(uint64_t key) { return (int32_t)(0xffffffffu - (uint32_t)key); }
 __device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int m) {
     return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, m);
@@ -177,8 +179,15 @@ __device__ __forceinline__ void lp_rank(const LpArgs& g, const uint64_t* cand, i
     const int k = g.k;
     for (int i = threadIdx.x; i < total; i += THREADS) {
         const uint64_t own = cand[i];
-        int rank = 0;
-        for (int q = 0; q < total; ++q) rank += cand[q] > own ? 1 : 0;
+        int rank = 0, q = 0;
+        for (; q + 8 <= total; q += 8) {     // eight at a time: their loads wait together
+            uint64_t other[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) other[j] = cand[q + j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rank += other[j] > own ? 1 : 0;
+        }
+        for (; q < total; ++q) rank += cand[q] > own ? 1 : 0;
         if (rank < k) {
             if (g.part) {
                 g.keys[((long)row * g.S + piece) * k + rank] = own;
@@ -209,10 +218,13 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
             for (int j = 0; j < VEC; ++j) hit |= !(LpIo<T>::get(raw[i], j) < least) ? 1u << j : 0u;
             if (e < n) {
                 for (; hit; hit &= hit - 1) {
-                    const int x = e + __builtin_ctz(hit);
-                    if (x < n) {
+                    const int at_j = __builtin_ctz(hit);
+                    float x = 0.f;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) x = j == at_j ? LpIo<T>::get(raw[i], j) : x;
+                    if (e + at_j < n) {
                         const int at = atomicAdd(count, 1);
-                        if (at < LP_FEW) cand[at] = lp_key(LpIo<T>::one(z, x), lo + x);
+                        if (at < LP_FEW) cand[at] = lp_key(x, lo + e + at_j);
                     }
                 }
             }
@@ -323,12 +335,11 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
     // what the first wave finds out for all: the row's sums, and the least value of a candidate
     __shared__ float red[3][WAVES], group[64], joined[4];
     __shared__ int count;
-    constexpr int GL = THREADS / 64;         // lanes of the 64 groups: one, a quad or a row of 16
+    constexpr int GL = THREADS / 64;         // lanes of the 64 groups: 1, 2, 4, 8 or a row of 16
     float group_m = lane_m;
-    if constexpr (GL >= 4) {
-        group_m = fmaxf(group_m, dpp_f<DPP_XOR1>(group_m));
-        group_m = fmaxf(group_m, dpp_f<DPP_XOR2>(group_m));
-    }
+    if constexpr (GL >= 2) group_m = fmaxf(group_m, dpp_f<DPP_XOR1>(group_m));
+    if constexpr (GL >= 4) group_m = fmaxf(group_m, dpp_f<DPP_XOR2>(group_m));
+    if constexpr (GL >= 8) group_m = fmaxf(group_m, dpp_f<DPP_HALF_MIRROR>(group_m));
     if constexpr (GL == 16) group_m = row_m;
     if constexpr (WAVES > 1) {
         if (lane == 0) {
@@ -346,17 +357,15 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
             v = lp_join(v, c);
         }
         float least = 0.f;
-        if constexpr (MODE == LP_TOP) {      // k-th largest of 64: every lane counts what is above and what is not below its own
-            const float own = WAVES > 1 ? group[lane] : group_m;
-            int above = 0, reach = 0;
-#pragma unroll 8
-            for (int q = 0; q < 64; ++q) {
-                const float other = lane_f(own, q);
-                above += other > own ? 1 : 0;
-                reach += other >= own ? 1 : 0;
+        if constexpr (MODE == LP_TOP) {      // the k-th largest of 64, bit by bit: the largest number that k of them reach
+            const uint32_t own = lp_order(WAVES > 1 ? group[lane] : group_m);
+            uint32_t kth = 0;
+#pragma unroll
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t probe = kth | 1u << bit;
+                if ((int)__popcll(__ballot(own >= probe)) >= g.k) kth = probe;
             }
-            const uint64_t hit = __ballot(above < g.k && reach >= g.k);
-            least = lane_f(own, __builtin_ctzll(hit));
+            least = lp_from_order(kth);
             if (lane == 0) count = 0;
         }
         if (lane == 0) {
@@ -504,11 +513,12 @@ struct LpPlan { int threads, S, chunk; };
 static LpPlan lp_plan(int vec, int V, int k) {
     LpPlan p;
     const int lane = LP_NV * vec;
-    p.threads = V <= 64 * lane ? 64 : V <= 256 * lane ? 256 : 1024;
+    p.threads = 64;                          // the fewest lanes that hold the row
+    while (p.threads < 1024 && V > p.threads * lane) p.threads *= 2;
     // candidates of k groups have to fit 60 KiB of LDS: k x (group's elements) x 8 B
     long cap = (long)p.threads * lane;
     if (k > 0) {
-        const int gl = p.threads <= 256 ? 1 : 4;
+        const int gl = p.threads <= 256 ? 1 : p.threads / 256;
         const int per = (int)(60 * 1024 / 8 / k / gl) / vec * vec;       // elements a lane may hold
         if (per < lane) cap = (long)p.threads * per;
     }
@@ -518,7 +528,7 @@ static LpPlan lp_plan(int vec, int V, int k) {
     return p;
 }
 static size_t lp_cand_bytes(const LpPlan& p, int vec, int k) {
-    const int gl = p.threads <= 256 ? 1 : 4;
+    const int gl = p.threads <= 256 ? 1 : p.threads / 256;
     const size_t b = (size_t)k * gl * cdiv(p.chunk, (long)p.threads * vec) * vec * 8;
     return b > LP_FEW * 8 ? b : LP_FEW * 8;
 }
@@ -539,7 +549,9 @@ template <typename T, int MODE>
 static int lp_launch(LpArgs& g, const LpPlan& p, size_t lds, const char* what, hipStream_t s) {
     return lp_rows(g, g.S, p.threads, what, [&](dim3 grid) {
         if (p.threads == 64) hipLaunchKernelGGL((logprob_kernel<T, 64, MODE>), grid, dim3(64), lds, s, g);
+        else if (p.threads == 128) hipLaunchKernelGGL((logprob_kernel<T, 128, MODE>), grid, dim3(128), lds, s, g);
         else if (p.threads == 256) hipLaunchKernelGGL((logprob_kernel<T, 256, MODE>), grid, dim3(256), lds, s, g);
+        else if (p.threads == 512) hipLaunchKernelGGL((logprob_kernel<T, 512, MODE>), grid, dim3(512), lds, s, g);
         else hipLaunchKernelGGL((logprob_kernel<T, 1024, MODE>), grid, dim3(1024), lds, s, g);
     });
 }
