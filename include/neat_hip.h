@@ -374,8 +374,8 @@ int neat_token_logprobs(const void* logits, long ld, int dtype, const int64_t* t
 int neat_token_logprobs_bwd(const void* logits, long ld, int dtype, const int64_t* target, const float* stats,
                             const float* dlogp, const float* dentropy, float scale, void* dlogits, long ld_out, int R, int V,
                             void* stream);
-/* Both, for weights that are known beforehand: one reading of rows that fit a workgroup's registers (V <= 32 768 f32, 65 536
- * bf16), else the two calls above (stats is then required; ws as for k = 0). */
+/* Both, for weights that are known beforehand: one reading of rows that fit a workgroup's registers (V <= 65 536), else the
+ * two calls above (stats is then required; ws as for k = 0). */
 int neat_token_logprobs_fwd_bwd(const void* logits, long ld, int dtype, const int64_t* target, const float* dlogp,
                                 const float* dentropy, float scale, float* logp, float* entropy, float* stats, void* dlogits,
                                 long ld_out, int R, int V, void* ws, void* stream);

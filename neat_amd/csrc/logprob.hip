@@ -16,8 +16,9 @@
 // k-th largest of up to 256 groups' keys leaves at most k groups' elements, for which there is room.
 //
 // Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 186 us (974 MB, 5.2 TB/s), 2 000 x 25 014 fp32
-// with 10 alternatives 45 us (200 MB, 4.4 TB/s; the ranking of one row runs under the loads of another).  One row of 49 408 with
-// 5 alternatives: 10 us, half of it the exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining
+// with 10 alternatives 42 us (200 MB, 4.8 TB/s; the ranking of one row runs under the loads of another).  bf16 rows with
+// alternatives are bound by the vector ALU (3 to 4.5 TB/s).  One row of 49 408 with 5 alternatives: 9 us, half of it the
+// exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining
 // launch takes 1 us with them, so rows are cut only where they do not fit.
 #include "wave.h"
 
@@ -219,9 +220,13 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
             if (e < n) {
                 for (; hit; hit &= hit - 1) {
                     const int at_j = __builtin_ctz(hit);
-                    float x = 0.f;
+                    float x = 0.f;           // eight ways to choose from spill at 64 registers: asked from the cache again
+                    if constexpr (VEC == 4 || THREADS < 1024) {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) x = j == at_j ? LpIo<T>::get(raw[i], j) : x;
+                        for (int j = 0; j < VEC; ++j) x = j == at_j ? LpIo<T>::get(raw[i], j) : x;
+                    } else if (e + at_j < n) {
+                        x = LpIo<T>::one(z, e + at_j);
+                    }
                     if (e + at_j < n) {
                         const int at = atomicAdd(count, 1);
                         if (at < LP_FEW) cand[at] = lp_key(x, lo + e + at_j);
@@ -285,8 +290,8 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
 
 // One workgroup, one row (or one piece of it).  1 024 lanes: at most 64 registers, so that two rows share a CU and one loads
 // while the other computes.
-template <typename T, int THREADS, int MODE>
-__global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kernel(LpArgs g) {
+template <typename T, int THREADS, int MODE, int NV = LP_NV>
+__global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1) void logprob_kernel(LpArgs g) {
     constexpr int VEC = LpIo<T>::VEC, WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = g.row0 + blockIdx.x / g.S, piece = blockIdx.x % g.S;
@@ -294,9 +299,9 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
     const T* z = static_cast<const T*>(g.z) + (long)row * g.ld + lo;
     const float c = g.scale * LOG2E;
 
-    u32x4 raw[LP_NV];
+    u32x4 raw[NV];
 #pragma unroll
-    for (int i = 0; i < LP_NV; ++i) {
+    for (int i = 0; i < NV; ++i) {
         const int e = (tid + i * THREADS) * VEC;
         raw[i] = u32x4{LpIo<T>::NEG, LpIo<T>::NEG, LpIo<T>::NEG, LpIo<T>::NEG};
         if (e + VEC <= n) {
@@ -309,7 +314,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
     }
     float lane_m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < LP_NV; ++i) {
+    for (int i = 0; i < NV; ++i) {
         if (i * THREADS * VEC < n) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) lane_m = fmaxf(lane_m, LpIo<T>::get(raw[i], j));
@@ -320,7 +325,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
     const float m0 = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
 #pragma unroll
-    for (int i = 0; i < LP_NV; ++i) {
+    for (int i = 0; i < NV; ++i) {
         if (i * THREADS * VEC < n) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -396,7 +401,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 1) void logprob_kern
         T* dz = static_cast<T*>(g.dz) + (long)row * g.ldz;
         if (WAVES > 1) __syncthreads();      // dz may be the logits: lane 0 has read the target's before anything is written
 #pragma unroll
-        for (int i = 0; i < LP_NV; ++i) {
+        for (int i = 0; i < NV; ++i) {
             const int e = (tid + i * THREADS) * VEC;
             if (e < n) {
                 const u32x4 o = lp_grad_vec<T>(raw[i], q, c, e);
@@ -509,10 +514,14 @@ __global__ __launch_bounds__(LPB_THREADS) void logprob_bwd_kernel(LpArgs g) {
 }
 
 // how a row is laid over workgroups: lanes per workgroup, pieces per row and their length
-struct LpPlan { int threads, S, chunk; };
-static LpPlan lp_plan(int vec, int V, int k) {
+struct LpPlan { int threads, S, chunk, nv; };
+static LpPlan lp_plan(int vec, int V, int k, bool grad = false) {
     LpPlan p;
-    const int lane = LP_NV * vec;
+    int lane = LP_NV * vec;
+    // a gradient's second reading costs more than a CU with one workgroup loses (400 MB of fp32 rows of 49 408: 3.8 TB/s cut and
+    // read twice, 5.4 so): fp32 rows that need it get twice the registers
+    if (grad && vec == 4 && V > 1024 * lane && V <= 2 * 1024 * lane) lane *= 2;
+    p.nv = lane / vec;
     p.threads = 64;                          // the fewest lanes that hold the row
     while (p.threads < 1024 && V > p.threads * lane) p.threads *= 2;
     // candidates of k groups have to fit 60 KiB of LDS: k x (group's elements) x 8 B
@@ -552,6 +561,10 @@ static int lp_launch(LpArgs& g, const LpPlan& p, size_t lds, const char* what, h
         else if (p.threads == 128) hipLaunchKernelGGL((logprob_kernel<T, 128, MODE>), grid, dim3(128), lds, s, g);
         else if (p.threads == 256) hipLaunchKernelGGL((logprob_kernel<T, 256, MODE>), grid, dim3(256), lds, s, g);
         else if (p.threads == 512) hipLaunchKernelGGL((logprob_kernel<T, 512, MODE>), grid, dim3(512), lds, s, g);
+        else if constexpr (MODE == LP_GRAD && sizeof(T) == 4) {
+            if (p.nv > LP_NV) hipLaunchKernelGGL((logprob_kernel<T, 1024, MODE, 2 * LP_NV>), grid, dim3(1024), lds, s, g);
+            else hipLaunchKernelGGL((logprob_kernel<T, 1024, MODE>), grid, dim3(1024), lds, s, g);
+        }
         else hipLaunchKernelGGL((logprob_kernel<T, 1024, MODE>), grid, dim3(1024), lds, s, g);
     });
 }
@@ -647,7 +660,7 @@ extern "C" int neat_token_logprobs_fwd_bwd(const void* logits, long ld, int dtyp
     NEAT_REQUIRE(R <= 1 || ld_out >= V, NEAT_ERR_SHAPE, "neat_token_logprobs_fwd_bwd: output row pitch %ld below V=%d", ld_out, V);
     NEAT_REQUIRE(((uintptr_t)dlogits & (dtype == NEAT_F32 ? 3 : 1)) == 0, NEAT_ERR_ARG,
                  "neat_token_logprobs_fwd_bwd: gradient is not aligned to its elements");
-    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, 0);
+    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, 0, true);
     if (p.S > 1) {                            // longer than a workgroup's registers: two passes
         NEAT_REQUIRE(stats, NEAT_ERR_ARG, "neat_token_logprobs_fwd_bwd: rows of %d need stats", V);
         if (int rc = neat_token_logprobs(logits, ld, dtype, target, scale, 0, logp, entropy, stats, nullptr, nullptr, R, V, ws,
