@@ -364,7 +364,7 @@ int neat_comm_destroy(void);
  * logp, entropy, stats may be NULL; target may be NULL with logp.  -inf logits are masked: a row of nothing else has logp =
  * -inf, entropy 0, alternatives of -inf, gradient 0.  A NaN or +inf makes the row's numbers NaN; a NaN is never an
  * alternative.  ws: neat_token_logprobs_ws_bytes bytes of device memory, 16-B aligned (0: may be NULL).  V <= 2 097 152 (f32) /
- * 4 194 304 (bf16; alternatives: V up to 64 pieces of 57 344). */
+ * 4 194 304 (bf16). */
 long neat_token_logprobs_ws_bytes(int dtype, int R, int V, int k);
 int neat_token_logprobs(const void* logits, long ld, int dtype, const int64_t* target, float scale, int k, float* logp,
                         float* entropy, float* stats, float* top_logp, int32_t* top_idx, int R, int V, void* ws,

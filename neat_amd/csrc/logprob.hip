@@ -13,7 +13,7 @@
 // Alternatives: the k-th largest of 64 group maxima bounds the k-th largest value from below; the few values that reach it are
 // collected and ranked by counting (value, then lower index): no sort, and no atomic that matters to the result.  Where many
 // reach it (a row of few different values, or mostly masked), 64-bit keys (value, index) that never tie take its place: the
-// k-th largest of up to 256 groups' keys leaves at most k groups' elements, for which there is room.
+// k-th largest of 256 to 1 024 groups' keys leaves at most k groups' elements, for which there is room.
 //
 // Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 186 us (974 MB, 5.2 TB/s), 2 000 x 25 014 fp32
 // with 10 alternatives 42 us (200 MB, 4.8 TB/s; the ranking of one row runs under the loads of another).  bf16 rows with
@@ -171,6 +171,8 @@ __device__ __forceinline__ u32x4 lp_grad_vec(u32x4 raw, const LpGrad& q, float c
 
 enum { LP_SUMS = 0, LP_TOP = 1, LP_GRAD = 2 };
 
+// groups of the exact bound: parts of a lane's vectors
+template <int THREADS> struct LpGroups { static constexpr int PARTS = THREADS < 256 ? 256 / THREADS : 1; };
 constexpr int LP_FEW = 256;                  // candidates of the first bound that are ranked; more go by keys
 
 // the k largest of the `total` keys in `cand`, in order
@@ -206,7 +208,7 @@ __device__ __forceinline__ void lp_rank(const LpArgs& g, const uint64_t* cand, i
 template <typename T, int THREADS>
 __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, const u32x4 (&raw)[LP_NV], int row, int piece, int lo,
                                                 int n, float lane_m, float least, int* count, const LpRow& r, float s) {
-    constexpr int VEC = LpIo<T>::VEC, GROUPS = THREADS < 256 ? THREADS : 256, GL = THREADS / GROUPS;
+    constexpr int VEC = LpIo<T>::VEC;
     extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
     const int tid = threadIdx.x;
     // NaN counts as -inf, which is why the comparisons are turned round
@@ -241,43 +243,47 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
         lp_rank<THREADS>(g, cand, total, row, piece, r, s);
         return;
     }
-    // many values reach the bound: the same once more with keys that never tie, from memory (the row is in the caches)
+    // many values reach the bound: the same once more with keys that never tie, from memory (the row is in the caches).  A group
+    // is a lane's vectors, or a part of them where there are few lanes: the fewer elements it has, the less LDS its candidates
+    // need (64 lanes with whole lanes for groups: 16 KiB at k = 32, and only nine workgroups fit a CU)
+    constexpr int PARTS = LpGroups<THREADS>::PARTS, GROUPS = THREADS * PARTS, PER = LP_NV / PARTS;
     __shared__ uint64_t group[GROUPS];
     __shared__ uint64_t bound;
     __syncthreads();
-    uint64_t mine = 0;
-    for (int first = tid * VEC; first < n; first += THREADS * VEC) {
-        const int last = min(first + VEC, n);
-        for (int e = first; e < last; ++e) {
-            const uint64_t key = lp_key(LpIo<T>::one(z, e), lo + e);
-            mine = key > mine ? key : mine;
-        }
-    }
-    uint64_t best = mine;
+    uint64_t mine[PARTS];
 #pragma unroll
-    for (int o = 1; o < GL; o <<= 1) {
-        const uint64_t other = lp_shfl_xor(best, o);
-        best = other > best ? other : best;
+    for (int p = 0; p < PARTS; ++p) {
+        mine[p] = 0;
+        for (int i = p * PER; i < (p + 1) * PER; ++i) {
+            const int first = (tid + i * THREADS) * VEC, last = min(first + VEC, n);
+            for (int e = first; e < last; ++e) {
+                const uint64_t key = lp_key(LpIo<T>::one(z, e), lo + e);
+                mine[p] = key > mine[p] ? key : mine[p];
+            }
+        }
+        group[tid * PARTS + p] = mine[p];
     }
-    if (tid % GL == 0) group[tid / GL] = best;
     if (tid == 0) {
         bound = 0;
         *count = 0;
     }
     __syncthreads();
-    {                                        // the k-th largest group: the GL lanes of a group count its betters together
-        const uint64_t own = group[tid / GL];
-        int rank = 0;
-        for (int q = tid % GL; q < GROUPS; q += GL) rank += group[q] > own ? 1 : 0;
+    int rank[PARTS] = {};
+    for (int q = 0; q < GROUPS; ++q) {
+        const uint64_t other = group[q];
 #pragma unroll
-        for (int o = 1; o < GL; o <<= 1) rank += __shfl_xor(rank, o);
-        if (rank == g.k - 1 && own != 0 && tid % GL == 0) bound = own;       // fewer groups than k: everything is a candidate
+        for (int p = 0; p < PARTS; ++p) rank[p] += other > mine[p] ? 1 : 0;
     }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+        if (rank[p] == g.k - 1 && mine[p] != 0) bound = mine[p];             // fewer groups than k: everything is a candidate
     __syncthreads();
     const uint64_t floor_key = bound;
-    if (mine != 0 && mine >= floor_key) {
-        for (int first = tid * VEC; first < n; first += THREADS * VEC) {
-            const int last = min(first + VEC, n);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        if (mine[p] == 0 || mine[p] < floor_key) continue;
+        for (int i = p * PER; i < (p + 1) * PER; ++i) {
+            const int first = (tid + i * THREADS) * VEC, last = min(first + VEC, n);
             for (int e = first; e < last; ++e) {
                 const uint64_t key = lp_key(LpIo<T>::one(z, e), lo + e);
                 if (key >= floor_key) cand[atomicAdd(count, 1)] = key;
@@ -515,7 +521,7 @@ __global__ __launch_bounds__(LPB_THREADS) void logprob_bwd_kernel(LpArgs g) {
 
 // how a row is laid over workgroups: lanes per workgroup, pieces per row and their length
 struct LpPlan { int threads, S, chunk, nv; };
-static LpPlan lp_plan(int vec, int V, int k, bool grad = false) {
+static LpPlan lp_plan(int vec, int V, bool grad = false) {
     LpPlan p;
     int lane = LP_NV * vec;
     // a gradient's second reading costs more than a CU with one workgroup loses (400 MB of fp32 rows of 49 408: 3.8 TB/s cut and
@@ -525,20 +531,16 @@ static LpPlan lp_plan(int vec, int V, int k, bool grad = false) {
     p.threads = 64;                          // the fewest lanes that hold the row
     while (p.threads < 1024 && V > p.threads * lane) p.threads *= 2;
     // candidates of k groups have to fit 60 KiB of LDS: k x (group's elements) x 8 B
-    long cap = (long)p.threads * lane;
-    if (k > 0) {
-        const int gl = p.threads <= 256 ? 1 : p.threads / 256;
-        const int per = (int)(60 * 1024 / 8 / k / gl) / vec * vec;       // elements a lane may hold
-        if (per < lane) cap = (long)p.threads * per;
-    }
+    const long cap = (long)p.threads * lane;
     p.S = cdiv(V, cap);
     p.chunk = p.S == 1 ? V : (cdiv(V, p.S) + vec - 1) / vec * vec;
     p.S = cdiv(V, p.chunk);
     return p;
 }
+// candidates of k groups of the exact bound, or of the first one
 static size_t lp_cand_bytes(const LpPlan& p, int vec, int k) {
-    const int gl = p.threads <= 256 ? 1 : p.threads / 256;
-    const size_t b = (size_t)k * gl * cdiv(p.chunk, (long)p.threads * vec) * vec * 8;
+    const int parts = p.threads < 256 ? 256 / p.threads : 1, held = cdiv(p.chunk, (long)p.threads * vec);
+    const size_t b = (size_t)k * (held < LP_NV / parts ? held : LP_NV / parts) * vec * 8;
     return b > LP_FEW * 8 ? b : LP_FEW * 8;
 }
 static long lp_part_bytes(long R, const LpPlan& p) { return p.S == 1 ? 0 : (R * p.S * 16 + 255) / 256 * 256; }
@@ -605,7 +607,7 @@ using namespace neat;
 
 extern "C" long neat_token_logprobs_ws_bytes(int dtype, int R, int V, int k) {
     if (R <= 0 || V <= 0 || k < 0 || k > LP_MAX_K) return 0;
-    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, k);
+    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V);
     return p.S == 1 ? 0 : lp_part_bytes(R, p) + (long)R * p.S * k * 8;
 }
 
@@ -618,9 +620,7 @@ extern "C" int neat_token_logprobs(const void* logits, long ld, int dtype, const
                  LP_MAX_K, V);
     NEAT_REQUIRE(k == 0 || R == 0 || (top_logp && top_idx), NEAT_ERR_ARG, "neat_token_logprobs: null pointer (alternatives)");
     if (R == 0) return NEAT_OK;
-    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, k);
-    NEAT_REQUIRE(p.S <= LP_MAX_SPLIT, NEAT_ERR_SHAPE, "neat_token_logprobs: V=%d with k=%d needs %d pieces (at most %d)", V, k,
-                 p.S, LP_MAX_SPLIT);
+    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V);
     NEAT_REQUIRE(p.S == 1 || (ws && ((uintptr_t)ws & 15) == 0), NEAT_ERR_ARG,
                  "neat_token_logprobs: rows of %d need a 16-byte aligned workspace", V);
     LpArgs g{};
@@ -660,7 +660,7 @@ extern "C" int neat_token_logprobs_fwd_bwd(const void* logits, long ld, int dtyp
     NEAT_REQUIRE(R <= 1 || ld_out >= V, NEAT_ERR_SHAPE, "neat_token_logprobs_fwd_bwd: output row pitch %ld below V=%d", ld_out, V);
     NEAT_REQUIRE(((uintptr_t)dlogits & (dtype == NEAT_F32 ? 3 : 1)) == 0, NEAT_ERR_ARG,
                  "neat_token_logprobs_fwd_bwd: gradient is not aligned to its elements");
-    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, 0, true);
+    const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, true);
     if (p.S > 1) {                            // longer than a workgroup's registers: two passes
         NEAT_REQUIRE(stats, NEAT_ERR_ARG, "neat_token_logprobs_fwd_bwd: rows of %d need stats", V);
         if (int rc = neat_token_logprobs(logits, ld, dtype, target, scale, 0, logp, entropy, stats, nullptr, nullptr, R, V, ws,

@@ -72,7 +72,7 @@ def _lp(z=64, ld=100, dtype=0, target=64, scale=1.0, k=0, logp=64, top=64, idx=6
     (dict(k=-1), -1, "k=-1"), (dict(k=2, top=None), -2, "alternatives"), (dict(z=66), -2, "aligned"),
     (dict(scale=0.0), -2, "scale"), (dict(scale=-1.0), -2, "scale"), (dict(scale=float("nan")), -2, "scale"),
     (dict(scale=float("inf")), -2, "scale"), (dict(V=3_000_000, ld=3_000_000), -1, "above"),
-    (dict(V=100_000, ld=100_000, ws=None), -2, "workspace"), (dict(V=4_100_000, ld=4_100_000, dtype=1, k=32), -1, "pieces")])
+    (dict(V=100_000, ld=100_000, ws=None), -2, "workspace"), (dict(V=4_200_000, ld=4_200_000, dtype=1, k=32), -1, "above")])
 def test_token_logprobs_checks_before_launching(bad, rc, says):
     assert _lp(**bad) == rc
     assert says in lib.last_error()
