@@ -12,6 +12,7 @@ parameter groups, gradients that come and go -- with moments in 32 or in 8 bits 
 from __future__ import annotations
 
 import array
+import itertools
 import operator
 
 import torch
@@ -152,7 +153,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for i, ps, layout, steps in self._lists:
             grads = list(map(_grad_of, ps))
             at = None
-            if type(None) in set(map(type, grads)):
+            if any(map(operator.is_, grads, itertools.repeat(None))):
                 at = [k for k, g in enumerate(grads) if g is not None]
                 if not at:
                     continue
