@@ -92,28 +92,30 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         ps = [p for g in self.param_groups for p in g["params"]]
         if not ps:
             raise ValueError("MultiTensorAdamW: empty parameter list")
-        if len({id(p) for p in ps}) != len(ps):
+        if len(set(map(id, ps))) != len(ps):
             raise ValueError("MultiTensorAdamW: a parameter is listed twice")
         self.device = ps[0].device
-        if self.device.type != "cuda" or any(p.device != self.device for p in ps):
+        if self.device.type != "cuda" or len(set(map(torch.Tensor.get_device, ps))) != 1:
             raise RuntimeError("MultiTensorAdamW: parameters must be on one GPU")
-        for p in ps:
-            if p.dtype not in (torch.float32, torch.bfloat16):
-                raise RuntimeError(f"MultiTensorAdamW: parameters must be float32 or bfloat16, got {p.dtype}")
-            if not p.is_contiguous():
-                raise RuntimeError("MultiTensorAdamW: parameters must be contiguous")
+        dtypes = [p.dtype for p in ps]
+        if not set(dtypes) <= {torch.float32, torch.bfloat16}:
+            raise RuntimeError(f"MultiTensorAdamW: parameters must be float32 or bfloat16, got {set(dtypes)}")
+        if not all(map(torch.Tensor.is_contiguous, ps)):
+            raise RuntimeError("MultiTensorAdamW: parameters must be contiguous")
         self.state_bits = state_bits
-        blocks, self._first, self._numel = 0, {}, {}
-        for p in ps:
-            self._first[p], self._numel[p] = blocks, p.numel()
-            blocks += -(-p.numel() // ops.ADAMW_BLOCK)
-        # per group and type, what one call of the library updates: [group, parameters, their layout, their step counts]
-        self._lists = []
+        # by position in the list of all parameters: sizes, first blocks of the moments
+        self._params, self._numel = ps, list(map(torch.Tensor.numel, ps))
+        ends = list(itertools.accumulate([-(-n // ops.ADAMW_BLOCK) for n in self._numel]))
+        self._first, blocks = [0] + ends[:-1], ends[-1]
+        # per group and type, what one call of the library updates: [group, positions, parameters, layout, step counts]
+        self._lists, at = [], 0
         for i, g in enumerate(self.param_groups):
+            here = range(at, at + len(g["params"]))
+            at = here.stop
             for dt in (torch.float32, torch.bfloat16):
-                sub = [p for p in g["params"] if p.dtype == dt]
-                if sub:
-                    self._lists.append([i, sub, self._layout(sub), [0] * len(sub)])
+                pos = [k for k in here if dtypes[k] == dt]
+                if pos:
+                    self._lists.append([i, pos, [ps[k] for k in pos], self._layout(pos), [0] * len(pos)])
         dt = torch.uint8 if state_bits == 8 else torch.float32
         self._m = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
         self._v = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
@@ -127,10 +129,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             self.exp_avg_sq = self._v
         self._ready = True
 
-    def _layout(self, ps):
+    def _layout(self, pos):
         """(sizes, the same as a C array, first blocks of the moments as a C array)."""
-        sizes = [self._numel[p] for p in ps]
-        return sizes, array.array("q", sizes), array.array("q", [self._first[p] for p in ps])
+        sizes = [self._numel[k] for k in pos]
+        return sizes, array.array("q", sizes), array.array("q", [self._first[k] for k in pos])
 
     @staticmethod
     def _check_group(g):
@@ -150,7 +152,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for i, ps, layout, steps in self._lists:
+        for i, pos, ps, layout, steps in self._lists:
             grads = list(map(_grad_of, ps))
             at = None
             if any(map(operator.is_, grads, itertools.repeat(None))):
@@ -158,7 +160,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 if not at:
                     continue
                 ps, grads = [ps[k] for k in at], [grads[k] for k in at]
-                layout = self._layout(ps)
+                layout = self._layout([pos[k] for k in at])
             now = [k + 1 for k in (steps if at is None else [steps[j] for j in at])]
             group = self.param_groups[i]
             b1, b2 = group["betas"]
@@ -172,36 +174,40 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         return loss
 
     def _step_counts(self):
-        return {p: k for _, ps, _, steps in self._lists for p, k in zip(ps, steps)}
+        """Step counts by position."""
+        counts = [0] * len(self._params)
+        for _, pos, _, _, steps in self._lists:
+            for k, n in zip(pos, steps):
+                counts[k] = n
+        return counts
 
     def moments(self, p):
         """(exp_avg, exp_avg_sq) of one parameter in float32, in its shape, and its step count."""
-        if p not in self._first:
+        k = next((k for k, q in enumerate(self._params) if q is p), None)
+        if k is None:
             raise ValueError("MultiTensorAdamW: not one of this optimizer's parameters")
-        n, lo = self._numel[p], self._first[p]
+        n, lo = self._numel[k], self._first[k]
         rows = slice(lo, lo - (-n // ops.ADAMW_BLOCK))
         m, v = self.exp_avg[rows].float(), (self.exp_avg_root if self.state_bits == 8 else self._v)[rows].float()
         if self.state_bits == 8:
             m, v = m * self._ms[rows, None], (v * self._vs[rows, None]) ** 2
-        return m.reshape(-1)[:n].view(p.shape), v.reshape(-1)[:n].view(p.shape), self._step_counts()[p]
+        return m.reshape(-1)[:n].view(p.shape), v.reshape(-1)[:n].view(p.shape), self._step_counts()[k]
 
     def _buffers(self):
         return [t for t in (self._m, self._v, self._ms, self._vs) if t is not None]
 
     def state_dict(self):
         d = super().state_dict()
-        ps, steps = list(self._numel), self._step_counts()
-        d["state"] = {"state_bits": self.state_bits, "numels": [self._numel[p] for p in ps], "steps": [steps[p] for p in ps],
+        d["state"] = {"state_bits": self.state_bits, "numels": list(self._numel), "steps": self._step_counts(),
                       "buffers": self._buffers()}
         return d
 
     def load_state_dict(self, state_dict):
-        st, ps = state_dict["state"], list(self._numel)
-        if st.get("state_bits") != self.state_bits or st["numels"] != [self._numel[p] for p in ps]:
+        st = state_dict["state"]
+        if st.get("state_bits") != self.state_bits or st["numels"] != self._numel:
             raise ValueError("MultiTensorAdamW: the state belongs to other parameters or another state_bits")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for dst, src in zip(self._buffers(), st["buffers"]):
             dst.copy_(src)
-        steps = dict(zip(ps, st["steps"]))
-        for _, sub, _, held in self._lists:
-            held[:] = [int(steps[p]) for p in sub]
+        for _, pos, _, _, held in self._lists:
+            held[:] = [int(st["steps"][k]) for k in pos]

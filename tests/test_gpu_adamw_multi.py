@@ -78,7 +78,7 @@ def test_moments_in_32_bits(dtype, bucket):
             # the moments' own error enters the step: top instead of this step's gradient, k steps of it
             bound = _p_bound(want, ms[i], top[i] * k, d, k, dtype) + LR / (1 - B1 ** k) * ms[i].abs() / d * 3 * U * k * top[i] ** 2 / vs[i].clamp_min(1e-300)
             assert ((p.double() - want).abs() <= bound).all(), (i, k)
-    assert all((opt._m.view(-1)[lo * 256 + n:(lo + -(-n // 256)) * 256] == 0).all() for p in ps for lo, n in [(opt._first[p], p.numel())])
+    assert all((opt._m.view(-1)[lo * 256 + n:(lo + -(-n // 256)) * 256] == 0).all() for lo, n in zip(opt._first, opt._numel))
 
 
 @pytest.mark.parametrize("bucket", [False, True])
@@ -94,8 +94,7 @@ def test_moments_in_8_bits(dtype, bucket):
         ps[-1].grad[::300] *= 1e-7
         before = [p.detach().clone() for p in ps]
         held = []
-        for p in ps:
-            lo, n = opt._first[p], p.numel()
+        for p, lo, n in zip(ps, opt._first, opt._numel):
             rows = slice(lo, lo + -(-n // 256))
             m = opt.exp_avg[rows].double() * opt.exp_avg_scale[rows, None].double()
             r = opt.exp_avg_root[rows].double() * opt.exp_avg_root_scale[rows, None].double()
@@ -107,7 +106,7 @@ def test_moments_in_8_bits(dtype, bucket):
             bound = _p_bound(want, m, p.grad, d, k, dtype) + LR / (1 - B1 ** k) * m.abs() / d * 4 * U
             bound += LR / (1 - B1 ** k) / d * 2 * U * held[i][0].abs()
             assert ((p.double() - want).abs() <= bound).all(), (i, k)
-            lo, n = opt._first[p], p.numel()
+            lo, n = opt._first[i], p.numel()
             nb = -(-n // 256)
             for code, scale, x in ((opt.exp_avg, opt.exp_avg_scale, m), (opt.exp_avg_root, opt.exp_avg_root_scale, torch.sqrt(v))):
                 s = scale[lo:lo + nb].double()
