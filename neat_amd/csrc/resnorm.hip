@@ -16,8 +16,8 @@
 // left behind at each group's end in slot team + group: runs and groups advance together, so no two (team, group) pairs share a
 // slot, and a second launch adds each group's slots, and the column sums, in a fixed order: no atomics, equal bits on every run.
 //
-// Bound by HBM: 78 848 x 512 (bf16 branch, a gate per 77 rows) forward 92 us (484 MB, 5.2 TB/s), backward 140 us (727 MB, 5.2)
-// and 9 us for the sums; 50 000 x 1 280 forward 161 us.  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9 us) is the
+// Bound by HBM: 78 848 x 512 (bf16 branch, a gate per 77 rows) forward 90 us (484 MB, 5.4 TB/s), backward 140 us (727 MB, 5.2)
+// and 9 us for the sums; 50 000 x 1 280 forward 145 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9 us) is the
 // second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.3 us, a launch's latency.
 #include "wave.h"
 
@@ -485,17 +485,21 @@ static int rn_bwd_wpr(int cols, bool wide) {
     const int w = rn_bwd_wave_cols(wide);
     return cols <= w ? 1 : cols <= 2 * w ? 2 : cols <= 4 * w ? 4 : 8;
 }
-// As many workgroups as fit the chip's 256 CUs at once, by registers and LDS (forward every workgroup has four waves), and four
-// rows a team where there are that many.  One round of workgroups that all run: 30 M elements forward at 256 / 1 664 / 2 560 /
-// 4 096 columns 4.8 / 4.4 / 4.2 / 3.3 TB/s with 8 192 teams whatever fits, 5.6 / 5.6 / 5.4 / 5.3 so.
-static int rn_fwd_blocks(int rows, int cols, bool wide) {
-    const int wpr = rn_fwd_wpr(cols), per = wpr == 1 ? RN_FWD_WAVES : 1;
-    const int waves = rn_fwd_waves(cdiv(cols / 4, 64 * wpr), wide), by_lds = 160 * 1024 / (16 * cols + 64);
-    const int most = 256 * (by_lds < waves ? by_lds : waves);
-    const int all = cdiv(rows, per), few = all < 256 ? all : 256;
-    int b = cdiv(rows, per * 4);
-    b = b < few ? few : b;
-    return b < 1 ? 1 : b > most ? most : b;
+// Where all workgroups can run at once (by registers and LDS; forward every one has four waves) with at most four rows a team, as
+// few rows as that takes.  6 M bf16 elements at 768 columns with both norms 4.3 / 5.0 / 3.9 TB/s with one / two / four, 11 M 4.4 /
+// 4.8 / 5.0, 12 M at 1 024 columns 4.5 / 4.9 / 4.8 and 5.2 with the three that the rule takes.
+// Beyond that two: more leave the chip's last workgroups uneven, one loads the weights for every row.  40 M at 512 / 1 024 columns
+// 4.8 / 5.2 TB/s with one, 5.3 / 5.1 with two, 5.0 / 4.8 with four; 50 000 x 1 280 with one norm 147 / 146 / 156 us.
+// A workgroup that is one team and stages two norms' weights wants more rows for them: 40 M at 1 664 / 2 560 / 4 096 columns 4.8 /
+// 4.4 / 4.2 TB/s with two, 4.9 / 4.6 / 4.6 with four, 4.8 / 4.4 / 4.3 with six; 4 M at 4 096 2.5 with one, 3.1 with two.
+// At most 2^18 workgroups: rows times teams stay below the 2^52 that the row runs' quotients are exact for.
+static int rn_fwd_blocks(int rows, int cols, bool wide, bool post) {
+    const int wpr = rn_fwd_wpr(cols), all = cdiv(rows, wpr == 1 ? RN_FWD_WAVES : 1);
+    const int waves = rn_fwd_waves(cdiv(cols / 4, 64 * wpr), wide), by_lds = 160 * 1024 / ((post ? 16 : 8) * cols + 64);
+    const int few = cdiv(all, 256 * (by_lds < waves ? by_lds : waves));
+    const bool staged = wpr > 1 && post;
+    const int run = few > 4 ? (staged ? 4 : 2) : few == 1 && staged && all > 512 ? 2 : few, b = cdiv(all, run);
+    return b < 1 << 18 ? b : 1 << 18;
 }
 static int rn_bwd_blocks(int rows, int cols, bool wide) {
     const int wpr = rn_bwd_wpr(cols, wide), per = wpr == 1 ? RN_BWD_WAVES : 1;
@@ -599,7 +603,7 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     if (int rc = rn_check("neat_res_norm_fwd", a, dtype, kind)) return rc;
     if (rows == 0) return NEAT_OK;
     NEAT_REQUIRE(x && h && pre_w && x_out && y, NEAT_ERR_ARG, "neat_res_norm_fwd: null pointer");
-    const int blocks = rn_fwd_blocks(rows, cols, dtype == NEAT_F32);
+    const int blocks = rn_fwd_blocks(rows, cols, dtype == NEAT_F32, post_w != nullptr);
     a.teams = blocks * (rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1);
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
 }

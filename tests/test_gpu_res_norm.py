@@ -161,6 +161,17 @@ def test_more_rows_than_teams(rows, cols, dtype, gate):
     check(rows, cols, dtype, "ln", True, True, gate, seed=rows)
 
 
+def test_more_rows_than_the_largest_grid_has_teams_for():
+    """2.2 million short rows forward: several thousand more than two rows for each of the 2^20 teams."""
+    rows, cols = (1 << 21) + 50_003, 8
+    x, h, pre_b, p, _, _ = make(rows, cols, torch.bfloat16, "ln", True, True, None, 5)
+    x_out, y, stats = ops.res_norm_fwd(x, h, p["pre_w"], pre_b, eps=EPS, **{k: v for k, v in p.items() if k != "pre_w"})
+    for cut in (slice(0, 5000), slice(rows // 2, rows // 2 + 5000), slice(rows - 60_000, rows)):
+        got = ops.res_norm_fwd(x[cut].contiguous(), h[cut].contiguous(), p["pre_w"], pre_b, eps=EPS,
+                               **{k: v for k, v in p.items() if k != "pre_w"})
+        assert torch.equal(x_out[cut], got[0]) and torch.equal(y[cut], got[1]) and torch.equal(stats[:, cut], got[2])
+
+
 def test_far_from_zero_and_constant_rows():
     check(20, 512, torch.float32, "ln", True, True, None, seed=7, shift=300.0)
     x = torch.full((4, 256), 3.0, device=DEV)
