@@ -80,7 +80,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     ceil(numel / 256) blocks, in parameter order.  ``state_bits=8``: ``exp_avg`` and ``exp_avg_root`` (the SQUARE ROOT of
     the second moment) are e4m3 numbers [blocks, 256], each block times its power of two ``exp_avg_scale`` /
     ``exp_avg_root_scale`` [blocks]: 2 bytes an element instead of 8.  ``moments(p)`` gives one parameter's as it would be
-    in 32 bits.  A parameter whose ``.grad`` is None is left alone and its step count stays (as in torch)."""
+    in 32 bits.  A parameter whose ``.grad`` is None is left alone and its step count stays (as in torch).
+
+    The host looks at every tensor on every step (0.5 us each): for many small float32 tensors that may be re-pointed to one
+    buffer, ``AdamW`` above costs the host less."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         if state_bits not in (32, 8):
