@@ -41,7 +41,7 @@ struct AwLaunch {
     void *m, *v;
     float *ms, *vs;
     uint32_t count, units;
-    double omb1_64;                 // 1 - beta1 as the caller has it
+    double omb1_64, b2_64, omb2_64; // 1 - beta1, beta2, 1 - beta2 as the caller has them
     float decay, omb1, b2, omb2, eps;
     AwTensor t[AW_TENSORS];
 };
@@ -177,10 +177,25 @@ __device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 
                     m[k][j] = __uint_as_float((rest > 0.0) == (m[k][j] > 0.f) ? u + 1 : u - 1);
             }
     }
+    // A root is off by 2^-22 of itself at most (the square of a held root is exact; four roundings of the sum, halved, and the
+    // hardware's root).  Where that leaves two codes, squares in 64 bits decide between them: the codes are the exact roots'
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+        uint32_t code = to_e4m3(r[k] * (1.f - 0x1p-21f));
+        const uint32_t above = to_e4m3(r[k] * (1.f + 0x1p-21f));
+        if (__any(code != above)) {
+            asm volatile("");
+            const f32x4 lo = from_e4m3(code), hi = from_e4m3(above), was = from_e4m3(h.v[k]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double mid = 0.5 * ((double)lo[j] + (double)hi[j]) * (double)pow2i(re), root = (double)(was[j] * h.vs);
+                const double side = __builtin_fma(root * root, a.b2_64, (double)g[k][j] * (double)g[k][j] * a.omb2_64) - mid * mid;
+                if (lo[j] < hi[j]) r[k][j] = side > 0.0 ? hi[j] : side < 0.0 ? lo[j] : 0.5f * (lo[j] + hi[j]);
+            }
+            code = to_e4m3(r[k]);
+        }
         h.m[k] = to_e4m3(m[k]);
-        h.v[k] = to_e4m3(r[k]);
+        h.v[k] = code;
     }
     h.ms = pow2i(me);
     h.vs = pow2i(re);
@@ -213,14 +228,8 @@ __device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f
             m[k][j] = m[k][j] + (g[k][j] - m[k][j]) * a.omb1;
             v[k][j] = v[k][j] * a.b2 + g[k][j] * g[k][j] * a.omb2;
             // root and reciprocal of the hardware (one unit in the last place each): the step they scale is added to a
-            // parameter that is larger by orders of magnitude.  A root that is held in 8 bits is corrected once, so that next to
-            // no code is another than the exact root's
-            if constexpr (SMALL) {
-                const float y = __builtin_amdgcn_rsqf(fmaxf(v[k][j], 0x1p-126f)), x = v[k][j] * y;
-                r[k][j] = __builtin_fmaf(__builtin_fmaf(-x, x, v[k][j]), 0.5f * y, x);
-            } else {
-                r[k][j] = __builtin_amdgcn_sqrtf(v[k][j]);
-            }
+            // parameter that is larger by orders of magnitude
+            r[k][j] = __builtin_amdgcn_sqrtf(v[k][j]);
             odd |= __builtin_amdgcn_classf(v[k][j], 0x280);
         }
     }
@@ -389,6 +398,8 @@ extern "C" int neat_adamw_multi(int count, void* const* p, const void* const* g,
     a.decay = (float)(1.0 - lr * wd);
     a.omb1 = (float)(1.0 - beta1);
     a.omb1_64 = 1.0 - beta1;
+    a.b2_64 = beta2;
+    a.omb2_64 = 1.0 - beta2;
     a.b2 = (float)beta2;
     a.omb2 = (float)(1.0 - beta2);
     a.eps = (float)eps;

@@ -137,6 +137,27 @@ def test_codes_follow_nearest_even_like_torch():
     assert torch.equal(p.detach(), torch.zeros_like(p))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_codes_of_roots_are_those_of_the_exact_roots(dtype):
+    """16 million roots: next to no border between two codes is one rounded to the other side (32 bits alone round a few there).
+    Second moments are normal here, and no block's largest is at a border of the scales."""
+    n = 1 << 22
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV, dtype=dtype))
+    opt = MultiTensorAdamW([p], lr=0.0, betas=(B1, B2), weight_decay=0.0, state_bits=8)
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    was = torch.zeros(n // 256, 256, dtype=torch.float64, device=DEV)
+    for _ in range(4):
+        p.grad = (torch.randn(n, generator=gen, device=DEV) * torch.exp(torch.randn(n, generator=gen, device=DEV)) * 1e-3).to(dtype)
+        opt.step()
+        scale = opt.exp_avg_root_scale.view(-1, 1).double()
+        q = torch.sqrt(was ** 2 * B2 + p.grad.double().view(-1, 256) ** 2 * (1 - B2)) / scale
+        step = torch.exp2(torch.floor(torch.log2(q.clamp(min=2.0 ** -6))) - 3)
+        want = torch.where(q > 0, (torch.round(q / step) * step).clamp(min=2.0 ** -9), q)
+        got = opt.exp_avg_root.view(-1, 256).double()
+        assert torch.equal(got, want), int((got != want).sum())
+        was = got * scale
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_what_is_not_finite_stays_where_it_is(bits):
     p, q = _params([700, 700], torch.float32, 3)
