@@ -15,7 +15,7 @@
 // kernel arguments (96 tensors a launch): no table in device memory, so no copy to order behind other work and none to keep alive.
 //
 // Bound by HBM: 37.7 M fp32 parameters in 144 tensors 187 us (1 059 MB, 5.7 TB/s); in bf16 with 8-bit moments 82 us (381 MB, 4.6
-// TB/s, and about what the host needs to pass 144 tensors).  Small tensors are bound by the host: 6 us of 31 for 48 x 512.
+// TB/s).  Small tensors are bound by the host: 6 us of 15 for 48 x 512.
 #include <math.h>
 
 #include "common.h"

@@ -108,6 +108,23 @@ def load() -> C.CDLL:
     return _lib
 
 
+_step_list = None
+
+
+def step_list():
+    """neat_host_step_list of libneat_host.so (csrc/host.cpp), the package's helper that reads lists of tensors."""
+    global _step_list
+    if _step_list is None:
+        import torch  # noqa: F401  (the helper resolves against torch's libraries)
+        path = os.path.join(_HERE, "libneat_host.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} not found: build it with `make -C neat_amd/csrc`")
+        fn = C.PyDLL(path).neat_host_step_list
+        fn.restype, fn.argtypes = _I, [C.py_object, _L, _P, _I, _I, _P, _P, _P, _P]
+        _step_list = fn
+    return _step_list
+
+
 def last_error() -> str:
     return load().neat_last_error().decode()
 

@@ -684,7 +684,7 @@ _contiguous = torch.Tensor.is_contiguous
 def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd):
     """The launch behind adamw_multi, for moments that are known to hold tensors of ``sizes`` (list, and C array) at
     ``blocks_c``; it looks at all that a caller can change between two steps.  Every check is one ``map`` over the list: the
-    host needs 0.4 us a tensor, where 144 tensors of a text tower take the GPU 80 us."""
+    host needs 0.4 us a tensor."""
     count, first = len(params), params[0]
     dtype, index = first.dtype, first.get_device()
     if dtype not in _DTYPES:
@@ -701,12 +701,17 @@ def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, 
         raise RuntimeError("adamw_multi: all tensors must be on one device")
     if index < 0:
         raise RuntimeError("adamw_multi: expected GPU tensors (libneat_hip has no CPU path)")
+    p_c, g_c = array.array("Q", map(_ptr_of, params)), array.array("Q", map(_ptr_of, grads))
+    _adamw_launch(first.device, count, p_c, g_c, sizes_c, blocks_c, array.array("i", steps), dtype, m, v, m_scale, v_scale, lr, beta1,
+                  beta2, eps, wd)
+
+
+def _adamw_launch(device, count, p_c, g_c, sizes_c, blocks_c, steps_c, dtype, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd):
+    """The launch for lists that have been looked at, as C arrays."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_multi: the step counts are host values that a graph would replay unchanged: "
                            "capture the backward pass and step outside the graph")
-    p_c, g_c = array.array("Q", map(_ptr_of, params)), array.array("Q", map(_ptr_of, grads))
-    steps_c = array.array("i", steps)
-    _call_on(first.device, "neat_adamw_multi", count, p_c.buffer_info()[0], g_c.buffer_info()[0], sizes_c.buffer_info()[0],
+    _call_on(device, "neat_adamw_multi", count, p_c.buffer_info()[0], g_c.buffer_info()[0], sizes_c.buffer_info()[0],
              blocks_c.buffer_info()[0], steps_c.buffer_info()[0], _DTYPES[dtype], _p(m), _p(v), _p(m_scale, f32, "m_scale"),
              _p(v_scale, f32, "v_scale"), 8 if m.dtype == torch.uint8 else 32, lr, beta1, beta2, eps, wd)
 
