@@ -15,7 +15,8 @@
 // reach it (a row of few different values, or mostly masked), 64-bit keys (value, index) that never tie take its place: the
 // k-th largest of 256 to 1 024 groups' keys leaves at most k groups' elements, for which there is room.
 //
-// Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 186 us (974 MB, 5.2 TB/s), 2 000 x 25 014 fp32
+// Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 183 us (974 MB, 5.3 TB/s; the vector
+// ALU is as busy, nine tenths), 2 000 x 25 014 fp32
 // with 10 alternatives 42 us (200 MB, 4.8 TB/s; the ranking of one row runs under the loads of another).  bf16 rows with
 // alternatives are bound by the vector ALU (3 to 4.5 TB/s).  One row of 49 408 with 5 alternatives: 9 us, half of it the
 // exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining
@@ -304,6 +305,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1
     const int lo = piece * g.chunk, n = min(g.chunk, g.V - lo);
     const T* z = static_cast<const T*>(g.z) + (long)row * g.ld + lo;
     const float c = g.scale * LOG2E;
+    const int first = __builtin_amdgcn_readfirstlane(tid);     // the wave's first lane: waves skip what lies behind the row (187 -> 183 us)
 
     u32x4 raw[NV];
 #pragma unroll
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1
     float lane_m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (i * THREADS * VEC < n) {
+        if ((first + i * THREADS) * VEC < n) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) lane_m = fmaxf(lane_m, LpIo<T>::get(raw[i], j));
         }
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (i * THREADS * VEC < n) {
+        if ((first + i * THREADS) * VEC < n) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const float d = (LpIo<T>::get(raw[i], j) - m0) * c, e = __builtin_amdgcn_exp2f(d);
