@@ -15,12 +15,11 @@
 // reach it (a row of few different values, or mostly masked), 64-bit keys (value, index) that never tie take its place: the
 // k-th largest of 256 to 1 024 groups' keys leaves at most k groups' elements, for which there is room.
 //
-// Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 183 us (974 MB, 5.3 TB/s; the vector
-// ALU is as busy, nine tenths), 2 000 x 25 014 fp32
-// with 10 alternatives 42 us (200 MB, 4.8 TB/s; the ranking of one row runs under the loads of another).  bf16 rows with
-// alternatives are bound by the vector ALU (3 to 4.5 TB/s).  One row of 49 408 with 5 alternatives: 9 us, half of it the
-// exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining
-// launch takes 1 us with them, so rows are cut only where they do not fit.
+// Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 183 us (974 MB, 5.3 TB/s; the vector ALU is
+// nine tenths busy there), 2 000 x 25 014 fp32 with 10 alternatives 41 us (200 MB, 4.8 TB/s; the ranking of one row runs under the
+// loads of another).  bf16 rows with alternatives are bound by the vector ALU (10 of them: rows of 1 000 2.4, of 16 385 3.4, of
+// 49 408 3.9 TB/s).  One row of 49 408 with 5 alternatives: 9 us, half of it the exponentials of one CU.  Cutting it over 13 CUs
+// makes the sums 1 us faster and the joining launch takes 1 us with them, so rows are cut only where they do not fit.
 #include "wave.h"
 
 namespace neat {
@@ -211,11 +210,12 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
                                                 int n, float lane_m, float least, int* count, const LpRow& r, float s) {
     constexpr int VEC = LpIo<T>::VEC;
     extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, first = __builtin_amdgcn_readfirstlane(tid);
     // NaN counts as -inf, which is why the comparisons are turned round
     if (!(lane_m < least)) {
 #pragma unroll
         for (int i = 0; i < LP_NV; ++i) {
+            if ((first + i * THREADS) * VEC >= n) break;
             const int e = (tid + i * THREADS) * VEC;
             uint32_t hit = 0;
 #pragma unroll
@@ -223,8 +223,8 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
             if (e < n) {
                 for (; hit; hit &= hit - 1) {
                     const int at_j = __builtin_ctz(hit);
-                    float x = 0.f;           // eight ways to choose from spill at 64 registers: asked from the cache again
-                    if constexpr (VEC == 4 || THREADS < 1024) {
+                    float x = 0.f;           // eight ways to choose from take over 64 registers: asked from the cache again
+                    if constexpr (VEC == 4) {
 #pragma unroll
                         for (int j = 0; j < VEC; ++j) x = j == at_j ? LpIo<T>::get(raw[i], j) : x;
                     } else if (e + at_j < n) {
@@ -295,17 +295,17 @@ __device__ __forceinline__ void lp_alternatives(const LpArgs& g, const T* z, con
     lp_rank<THREADS>(g, cand, *count, row, piece, r, s);
 }
 
-// One workgroup, one row (or one piece of it).  1 024 lanes: at most 64 registers, so that two rows share a CU and one loads
-// while the other computes.
+// One workgroup, one row (or one piece of it).  At most 64 registers, so that eight waves share a SIMD and some load while others
+// compute (bf16 rows of 16 385 with 10 alternatives 3.1 TB/s with five waves, 3.4 with eight; of 1 000 2.3 and 2.4).
 template <typename T, int THREADS, int MODE, int NV = LP_NV>
-__global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1) void logprob_kernel(LpArgs g) {
+__global__ __launch_bounds__(THREADS, NV > LP_NV ? 4 : 8) void logprob_kernel(LpArgs g) {
     constexpr int VEC = LpIo<T>::VEC, WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = g.row0 + blockIdx.x / g.S, piece = blockIdx.x % g.S;
     const int lo = piece * g.chunk, n = min(g.chunk, g.V - lo);
     const T* z = static_cast<const T*>(g.z) + (long)row * g.ld + lo;
     const float c = g.scale * LOG2E;
-    const int first = __builtin_amdgcn_readfirstlane(tid);     // the wave's first lane: waves skip what lies behind the row (187 -> 183 us)
+    const int first = __builtin_amdgcn_readfirstlane(tid);     // a wave skips the vectors behind the row's end (187 -> 183 us)
 
     u32x4 raw[NV];
 #pragma unroll
@@ -370,14 +370,16 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? (NV > LP_NV ? 4 : 8) : 1
             v = lp_join(v, c);
         }
         float least = 0.f;
-        if constexpr (MODE == LP_TOP) {      // the k-th largest of 64, bit by bit: the largest number that k of them reach
+        if constexpr (MODE == LP_TOP) {      // the k-th largest of 64, bit by bit: the largest number that k of them reach.  bf16
+            // numbers have nothing in the low half, which lp_order turns round below zero
             const uint32_t own = lp_order(WAVES > 1 ? group[lane] : group_m);
             uint32_t kth = 0;
 #pragma unroll
-            for (int bit = 31; bit >= 0; --bit) {
+            for (int bit = 31; bit >= (VEC == 8 ? 16 : 0); --bit) {
                 const uint32_t probe = kth | 1u << bit;
                 if ((int)__popcll(__ballot(own >= probe)) >= g.k) kth = probe;
             }
+            if (VEC == 8 && !(kth & 0x80000000u)) kth |= 0xffffu;
             least = lp_from_order(kth);
             if (lane == 0) count = 0;
         }

@@ -17,8 +17,8 @@
 // slot, and a second launch adds each group's slots, and the column sums, in a fixed order: no atomics, equal bits on every run.
 //
 // Bound by HBM: 78 848 x 512 (bf16 branch, a gate per 77 rows) forward 90 us (484 MB, 5.4 TB/s), backward 140 us (727 MB, 5.2)
-// and 9 us for the sums; 50 000 x 1 280 forward 145 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9 us) is the
-// second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.3 us, a launch's latency.
+// and 9 us for the sums; 50 000 x 1 280 forward 145 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9
+// us) is the second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.3 us, a launch's latency.
 #include "wave.h"
 
 namespace neat {

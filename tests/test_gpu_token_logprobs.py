@@ -178,6 +178,26 @@ def test_ties_go_to_the_lowest_index(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [40, 1000, 9000, 49408])
+def test_alternatives_on_both_sides_of_zero(V, dtype):
+    """Rows below zero, rows whose k-th alternative is next to zero, and rows with fewer unmasked entries than alternatives."""
+    gen = torch.Generator(device=DEV).manual_seed(V)
+    z = torch.randn(6, V, generator=gen, device=DEV)
+    z[0] = -z[0].abs() - 1
+    z[1] = -z[1].abs() * 1e30
+    z[2] = torch.where(torch.arange(V, device=DEV) < 7, z[2].abs(), -z[2].abs())
+    z[3] = torch.where(torch.arange(V, device=DEV) % 9 == 0, z[3].abs() * 1e-30, -z[3].abs() * 1e-30)
+    z[4] = torch.where(torch.arange(V, device=DEV) < 3, z[4], NEG)
+    z[5] = -(torch.arange(V, device=DEV).float() + 1)
+    z = z.to(dtype)
+    for k in (1, 7, 8, 32):
+        _, _, _, top, idx = ops.token_logprobs(z, None, k=k)
+        want = ref64(z, None, 1.0, k)
+        assert torch.equal(idx.cpu().long(), want["idx"]), k
+        close(top, want["top"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [2048, 8192, 16384, 32768, 65536])
 def test_alternatives_that_one_lane_holds(V, dtype):
     """The largest values sit where single lanes, or single groups of lanes, read: the most candidates a row can have."""
