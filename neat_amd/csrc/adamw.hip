@@ -177,8 +177,9 @@ __device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 
                     m[k][j] = __uint_as_float((rest > 0.0) == (m[k][j] > 0.f) ? u + 1 : u - 1);
             }
     }
-    // A root is off by 2^-22 of itself at most (the square of a held root is exact; four roundings of the sum, halved, and the
-    // hardware's root).  Where that leaves two codes, squares in 64 bits decide between them: the codes are the exact roots'
+    // A normal second moment's root is off by 2^-22 of itself at most (the square of a held root is exact; four roundings of the
+    // sum, halved, and the hardware's root).  Where that leaves two codes, squares in 64 bits decide between them: the codes are
+    // the exact roots'
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         uint32_t code = to_e4m3(r[k] * (1.f - 0x1p-21f));

@@ -266,9 +266,9 @@ __global__ __launch_bounds__(WPR == 1 ? 64 * RN_FWD_WAVES : 64 * WPR, rn_fwd_wav
 
 // Waves a SIMD that the backward kernel's registers are kept to: two rows in flight a wave and fewer waves are faster than one
 // row and one wave more (14 851 x 768: 91 against 96 us in both directions).
-constexpr int rn_bwd_waves(int nch) { return nch == 1 ? 5 : nch == 2 ? 3 : 2; }
+constexpr int rn_bwd_waves(int nch) { return nch == 1 ? 4 : nch == 2 ? 3 : 2; }
 template <typename T, int WPR, int NCH, bool POST>
-__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_waves(NCH) - (sizeof(T) == 4 && NCH == 1)) void res_norm_bwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(WPR == 1 ? 64 * RN_BWD_WAVES : 64 * WPR, rn_bwd_waves(NCH)) void res_norm_bwd_kernel(RnArgs a) {
     constexpr int TEAMS = WPR == 1 ? RN_BWD_WAVES : 1, THREADS = 64 * WPR * TEAMS;
     __shared__ float red[2][2][8];
     // pre_w, post_w, post_b: [3][cols]; behind them a team's sum of gate times group sums [TEAMS][cols]; at the end the sums
@@ -501,10 +501,12 @@ static int rn_fwd_blocks(int rows, int cols, bool wide, bool post) {
     const int run = few > 4 ? (staged ? 4 : 2) : few == 1 && staged && all > 512 ? 2 : few, b = cdiv(all, run);
     return b < 1 << 18 ? b : 1 << 18;
 }
+// Backward every workgroup leaves sums behind: as many as run at once, whole ones on each of the 256 CUs, and two rows a team.  40 M
+// bf16 elements with both norms at 768 / 4 096 columns 4.5 / 4.3 TB/s with half as many, 5.1 / 4.9 so, 5.0 / 4.6 with twice as many
+// (4.1 at 4 096 with one and a half a CU; 20 M fp32 at 128 columns 3.3 with five workgroups a CU of which four run, 4.4 with four).
 static int rn_bwd_blocks(int rows, int cols, bool wide) {
     const int wpr = rn_bwd_wpr(cols, wide), per = wpr == 1 ? RN_BWD_WAVES : 1;
-    const int most = 256 * 4 * rn_bwd_waves(cdiv(cols / 4, 64 * wpr)) / (wpr * per);
-    const int b = cdiv(rows, per * 2);
+    const int most = 256 * (4 * rn_bwd_waves(cdiv(cols / 4, 64 * wpr)) / (wpr * per)), b = cdiv(rows, per * 2);
     return b < 1 ? 1 : b > most ? most : b;
 }
 
