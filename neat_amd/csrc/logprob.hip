@@ -18,7 +18,7 @@
 // Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 183 us (974 MB, 5.3 TB/s; the vector ALU is
 // nine tenths busy there), 2 000 x 25 014 fp32 with 10 alternatives 41 us (200 MB, 4.8 TB/s; the ranking of one row runs under the
 // loads of another).  bf16 rows with alternatives are bound by the vector ALU (10 of them: rows of 1 000 2.4, of 16 385 3.4, of
-// 49 408 3.9 TB/s).  One row of 49 408 with 5 alternatives: 9 us, half of it the exponentials of one CU.  Cutting it over 13 CUs
+// 49 408 3.9 TB/s).  One row of 49 408 with 5 alternatives: 8 us, half of it the exponentials of one CU.  Cutting it over 13 CUs
 // makes the sums 1 us faster and the joining launch takes 1 us with them, so rows are cut only where they do not fit.
 #include "wave.h"
 
