@@ -14,7 +14,7 @@
 // fp32 per row and load, one reduction for four blocks, and all loads of a unit in flight together.  Tensor addresses travel as
 // kernel arguments (96 tensors a launch): no table in device memory, so no copy to order behind other work and none to keep alive.
 //
-// Bound by HBM: 37.7 M fp32 parameters in 144 tensors 187 us (1 059 MB, 5.7 TB/s); in bf16 with 8-bit moments 82 us (381 MB, 4.6
+// Bound by HBM: 37.7 M fp32 parameters in 144 tensors 183 us (1 059 MB, 5.8 TB/s); in bf16 with 8-bit moments 80 us (381 MB, 4.7
 // TB/s).  Small tensors are bound by the host: 6 us of 15 for 48 x 512.
 #include <math.h>
 
@@ -120,7 +120,7 @@ template <> struct AwHeld<true> { uint32_t m[4], v[4]; float ms, vs; };
 
 // the scales of a row's new moments, and the moments as multiples of them
 __device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 (&v)[4], f32x4 (&r)[4], const f32x4 (&g)[4],
-                                          bool from_zero, const AwLaunch& a) {
+                                          const AwLaunch& a) {
     constexpr uint32_t INF = 0x7f800000u, TINY = 0x00800000u;
     uint32_t mm = 0, vm = 0;
 #pragma unroll
@@ -163,19 +163,35 @@ __device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 
             const float q = r[k][j] * ri, up = r[k][j] * 0x1p100f;
             r[k][j] = __builtin_amdgcn_fmed3f(q, up, 0x1p-9f);
         }
-    if (__any(from_zero)) {
-        asm volatile("");
-        // a moment that starts from zero is the one product g (1 - b1), and products of short gradients often land halfway
-        // between two codes only by their own rounding: what was rounded off (found in 64 bits) decides then
+    // A normal first moment is off by one rounding of itself and three of what is added to the old one: by 7 x 2^-24 of the larger of
+    // old and new at most.  Where that leaves two codes, the sign of its distance from their middle decides, which 64 bits give
+    // exactly (short numbers, and one product and sum in one rounding): the codes are the exact moments' on every step, not 32
+    // bits', which put moments of short gradients in the middle (bf16: 1 to 4 in 100).  An old moment is taken for 1 024 units of the
+    // new codes at most, so that never more than one middle is in reach: beyond that a block has cancelled, and the 32-bit moment
+    // with it
+    const float mr = h.ms * mi;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 4; ++k) {
+        const f32x4 was = from_e4m3(h.m[k]) * mr;
+        f32x4 off;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t u = __float_as_uint(m[k][j]);
-                const double rest = __builtin_fma((double)g[k][j], a.omb1_64, -(double)(g[k][j] * a.omb1));
-                if ((h.m[k] >> (8 * j) & 0x7fu) == 0u && m[k][j] != 0.f && (u & 0x7ffffu) == 0 && (rest > 0.0 || rest < 0.0))
-                    m[k][j] = __uint_as_float((rest > 0.0) == (m[k][j] > 0.f) ? u + 1 : u - 1);
+        for (int j = 0; j < 4; ++j)
+            off[j] = 0x1.8p-21f * __builtin_amdgcn_fmed3f(__builtin_fabsf(m[k][j]), __builtin_fabsf(was[j]), 1024.f);
+        uint32_t code = to_e4m3(m[k] - off);
+        const uint32_t above = to_e4m3(m[k] + off);
+        if (__any(code != above)) {
+            asm volatile("");                           // to be branched around, not computed along
+            const f32x4 lo = from_e4m3(code), hi = from_e4m3(above);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {               // in units of the new codes; one code: both ends of the median are it
+                const float mid = 0.5f * (lo[j] + hi[j]);
+                const double old = (double)was[j], grad = (double)(g[k][j] * mi);
+                const float side = (float)__builtin_fma(grad - old, a.omb1_64, old - (double)mid);
+                m[k][j] = __builtin_amdgcn_fmed3f(lo[j], hi[j], __builtin_fmaf(side, 0x1p100f, mid));
             }
+            code = to_e4m3(m[k]);
+        }
+        h.m[k] = code;
     }
     // A normal second moment's root is off by 2^-22 of itself at most (the square of a held root is exact; four roundings of the
     // sum, halved, and the hardware's root).  Where that leaves two codes, squares in 64 bits decide between them: the codes are
@@ -195,26 +211,24 @@ __device__ __forceinline__ void aw_encode(AwHeld<true>& h, f32x4 (&m)[4], f32x4 
             }
             code = to_e4m3(r[k]);
         }
-        h.m[k] = to_e4m3(m[k]);
         h.v[k] = code;
     }
     h.ms = pow2i(me);
     h.vs = pow2i(re);
 }
 
-template <bool SMALL>
+// put: stores p, which then needs no registers while the moments are rounded (168 otherwise, three waves a SIMD, and 88 us where
+// 80 are measured)
+template <bool SMALL, typename F>
 __device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f32x4 (&g)[4], const AwLaunch& a,
-                                        const AwTensor& t) {
+                                        const AwTensor& t, F&& put) {
     f32x4 m[4], v[4], r[4];
-    uint32_t zeros = 0;
     bool odd = false;                                   // a moment that is subnormal or infinite
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if constexpr (SMALL) {
             m[k] = from_e4m3(h.m[k]);
             v[k] = from_e4m3(h.v[k]);
-            const uint32_t w = h.m[k] & 0x7f7f7f7fu;    // a byte of zeros: a code that stands for zero
-            zeros |= (w - 0x01010101u) & ~w;
         } else {
             m[k] = h.m[k];
             v[k] = h.v[k];
@@ -249,8 +263,9 @@ __device__ __forceinline__ void aw_step(AwHeld<SMALL>& h, f32x4 (&p)[4], const f
             p[k][j] = __builtin_fmaf(-t.step_size, u, p[k][j] * a.decay);
         }
     }
+    put();
     if constexpr (SMALL) {
-        aw_encode(h, m, v, r, g, (zeros & 0x80808080u) != 0u, a);
+        aw_encode(h, m, v, r, g, a);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -300,8 +315,9 @@ __device__ __forceinline__ void aw_store(const AwHeld<SMALL>& h, const AwLaunch&
     }
 }
 
+// 128 registers for 8-bit moments: four waves a SIMD
 template <typename T, bool SMALL>
-__global__ __launch_bounds__(64 * AW_WAVES) void adamw_multi_kernel(AwLaunch a) {
+__global__ __launch_bounds__(64 * AW_WAVES, SMALL ? 4 : 1) void adamw_multi_kernel(AwLaunch a) {
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * AW_WAVES + (threadIdx.x >> 6));
     if (unit >= a.units) return;
     uint32_t lo = 0, hi = a.count;                      // the tensor of this unit: the last one with unit0 <= unit
@@ -322,9 +338,10 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_multi_kernel(AwLaunch a) 
             p[k] = AwIo<T>::load(t.p, i + 64 * k);
         }
         aw_load<SMALL>(h, a, t.state_block + b, at);
-        aw_step<SMALL>(h, p, g, a, t);
+        aw_step<SMALL>(h, p, g, a, t, [&] {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) AwIo<T>::store(t.p, i + 64 * k, p[k]);
+            for (int k = 0; k < 4; ++k) AwIo<T>::store(t.p, i + 64 * k, p[k]);
+        });
         aw_store<SMALL>(h, a, t.state_block + b, at);
         return;
     }
@@ -353,19 +370,20 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_multi_kernel(AwLaunch a) 
                 }
         }
     }
-    aw_step<SMALL>(h, p, g, a, t);
-    if (mine) aw_store<SMALL>(h, a, t.state_block + b, at);
+    aw_step<SMALL>(h, p, g, a, t, [&] {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const long x = i + 64 * k;
-        if (x + 4 <= n) {
-            AwIo<T>::store(t.p, x, p[k]);
-        } else {
+        for (int k = 0; k < 4; ++k) {
+            const long x = i + 64 * k;
+            if (x + 4 <= n) {
+                AwIo<T>::store(t.p, x, p[k]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 3; ++j)
-                if (x + j < n) AwIo<T>::store1(t.p, x + j, p[k][j]);
+                for (int j = 0; j < 3; ++j)
+                    if (x + j < n) AwIo<T>::store1(t.p, x + j, p[k][j]);
+            }
         }
-    }
+    });
+    if (mine) aw_store<SMALL>(h, a, t.state_block + b, at);
 }
 
 }  // namespace neat
