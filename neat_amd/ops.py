@@ -672,8 +672,9 @@ def adamw_multi(params, grads, state_blocks, steps, m, v, m_scale=None, v_scale=
         for t, nm in ((m_scale, "m_scale"), (v_scale, "v_scale")):
             if t is None or tuple(t.shape) != (blocks,) or t.device != device:
                 raise RuntimeError(f"adamw_multi: {nm} must be float32 [{blocks}] on the parameters' device")
-    _adamw_multi(params, grads, sizes, array.array("q", sizes), array.array("q", state_blocks), steps, m, v,
-                 m_scale, v_scale, lr, beta1, beta2, eps, wd)
+    p_c, g_c, held = _adamw_addresses(params, grads, sizes)
+    _adamw_launch(device, count, p_c, g_c, array.array("q", sizes), array.array("q", state_blocks), array.array("i", steps),
+                  params[0].dtype, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd)
 
 
 _dtype_of, _ptr_of, _numel_of, _device_of = operator.attrgetter("dtype"), torch.Tensor.data_ptr, torch.Tensor.numel, \
@@ -681,11 +682,11 @@ _dtype_of, _ptr_of, _numel_of, _device_of = operator.attrgetter("dtype"), torch.
 _contiguous = torch.Tensor.is_contiguous
 
 
-def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd):
-    """The launch behind adamw_multi, for moments that are known to hold tensors of ``sizes`` (list, and C array) at
-    ``blocks_c``; it looks at all that a caller can change between two steps.  Every check is one ``map`` over the list: the
-    host needs 0.4 us a tensor."""
-    count, first = len(params), params[0]
+def _adamw_addresses(params, grads, sizes):
+    """(addresses of the parameters, of the gradients, the gradients they belong to) for a launch whose moments are laid out for
+    tensors of ``sizes``; it looks at all that a caller can change between two steps, and raises before anything is launched.
+    Every check is one ``map`` over the list: the host needs 0.4 us a tensor."""
+    first = params[0]
     dtype, index = first.dtype, first.get_device()
     if dtype not in _DTYPES:
         raise RuntimeError(f"adamw_multi: parameters must be float32 or bfloat16, got {dtype}")
@@ -693,17 +694,15 @@ def _adamw_multi(params, grads, sizes, sizes_c, blocks_c, steps, m, v, m_scale, 
         raise RuntimeError(f"adamw_multi: parameters and gradients must all be {dtype}")
     if not all(map(_contiguous, params)):
         raise RuntimeError("adamw_multi: parameters must be contiguous")
-    if not all(map(_contiguous, grads)):
-        grads = [t.contiguous() for t in grads]
     if list(map(_numel_of, params)) != sizes or list(map(_numel_of, grads)) != sizes:
         raise RuntimeError("adamw_multi: a gradient or parameter differs in size from what the moments were laid out for")
     if set(map(_device_of, params)) != {index} or set(map(_device_of, grads)) != {index}:
         raise RuntimeError("adamw_multi: all tensors must be on one device")
     if index < 0:
         raise RuntimeError("adamw_multi: expected GPU tensors (libneat_hip has no CPU path)")
-    p_c, g_c = array.array("Q", map(_ptr_of, params)), array.array("Q", map(_ptr_of, grads))
-    _adamw_launch(first.device, count, p_c, g_c, sizes_c, blocks_c, array.array("i", steps), dtype, m, v, m_scale, v_scale, lr, beta1,
-                  beta2, eps, wd)
+    if not all(map(_contiguous, grads)):
+        grads = [t.contiguous() for t in grads]
+    return array.array("Q", map(_ptr_of, params)), array.array("Q", map(_ptr_of, grads)), grads
 
 
 def _adamw_launch(device, count, p_c, g_c, sizes_c, blocks_c, steps_c, dtype, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd):

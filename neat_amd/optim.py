@@ -159,23 +159,33 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # every list is looked at before the first one is launched: a step that is refused has changed nothing
+        calls = []
         for i, dt, pos, ps, layout, steps in self._lists:
             group = self.param_groups[i]
             b1, b2 = group["betas"]
-            rest = (self._m, self._v, self._ms, self._vs, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-                    float(group["weight_decay"]))
+            rates = float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"])
             n, (_, sizes_c, blocks_c) = len(ps), layout
             p_c, g_c, now = array.array("Q", bytes(8 * n)), array.array("Q", bytes(8 * n)), array.array("i", bytes(4 * n))
             # the common step: every parameter has a gradient, and all are as they were laid out
             if lib.step_list()(ps, n, _at(sizes_c), dt == torch.bfloat16, self.device.index, _at(steps), _at(p_c), _at(g_c), _at(now)):
-                ops._adamw_launch(self.device, n, p_c, g_c, sizes_c, blocks_c, now, dt, *rest)
-                steps[:] = now
+                calls.append((n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, None, None))
                 continue
             grads = list(map(_grad_of, ps))
             at = [k for k, g in enumerate(grads) if g is not None]
             if at:
-                now = [steps[k] + 1 for k in at]
-                ops._adamw_multi([ps[k] for k in at], [grads[k] for k in at], *self._layout([pos[k] for k in at]), now, *rest)
+                sizes, sizes_c, blocks_c = self._layout([pos[k] for k in at])
+                some = [ps[k] for k in at]
+                if some[0].device != self.device:
+                    raise RuntimeError(f"MultiTensorAdamW: parameters must stay on {self.device}, where the moments are")
+                p_c, g_c, held = ops._adamw_addresses(some, [grads[k] for k in at], sizes)
+                now = array.array("i", [steps[k] + 1 for k in at])
+                calls.append((len(at), p_c, g_c, sizes_c, blocks_c, now, some[0].dtype, rates, steps, at, held))
+        for n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, at, _ in calls:
+            ops._adamw_launch(self.device, n, p_c, g_c, sizes_c, blocks_c, now, dt, self._m, self._v, self._ms, self._vs, *rates)
+            if at is None:
+                steps[:] = now
+            else:
                 for k, c in zip(at, now):
                     steps[k] = c
         return loss
