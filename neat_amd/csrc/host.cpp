@@ -38,3 +38,16 @@ extern "C" int neat_host_step_list(PyObject* params, int64_t count, const int64_
     }
     return 1;
 }
+
+// Says to autograd that the tensors in the list ``params`` (of the kind that neat_host_step_list takes) have been written: a backward
+// pass that saved one of them raises an error instead of using what is there now.
+extern "C" void neat_host_written(PyObject* params) {
+    if (!PyList_CheckExact(params)) return;
+    const Py_ssize_t n = PyList_GET_SIZE(params);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* const o = PyList_GET_ITEM(params, i);
+        if (!THPVariable_Check(o)) continue;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();     // inference tensors have no version
+    }
+}

@@ -108,21 +108,32 @@ def load() -> C.CDLL:
     return _lib
 
 
-_step_list = None
+_host = None
 
 
-def step_list():
-    """neat_host_step_list of libneat_host.so (csrc/host.cpp), the package's helper that reads lists of tensors."""
-    global _step_list
-    if _step_list is None:
+def _host_lib() -> C.PyDLL:
+    """libneat_host.so (csrc/host.cpp), the package's helper that reads lists of tensors."""
+    global _host
+    if _host is None:
         import torch  # noqa: F401  (the helper resolves against torch's libraries)
         path = os.path.join(_HERE, "libneat_host.so")
         if not os.path.exists(path):
             raise RuntimeError(f"{path} not found: build it with `make -C neat_amd/csrc`")
-        fn = C.PyDLL(path).neat_host_step_list
-        fn.restype, fn.argtypes = _I, [C.py_object, _L, _P, _I, _I, _P, _P, _P, _P]
-        _step_list = fn
-    return _step_list
+        dll = C.PyDLL(path)
+        dll.neat_host_step_list.restype, dll.neat_host_step_list.argtypes = _I, [C.py_object, _L, _P, _I, _I, _P, _P, _P, _P]
+        dll.neat_host_written.restype, dll.neat_host_written.argtypes = None, [C.py_object]
+        _host = dll
+    return _host
+
+
+def step_list():
+    """neat_host_step_list: addresses, gradients and step counts of a list of tensors."""
+    return _host_lib().neat_host_step_list
+
+
+def written():
+    """neat_host_written: says to autograd that the tensors in a list have been written."""
+    return _host_lib().neat_host_written
 
 
 def last_error() -> str:

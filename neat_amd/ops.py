@@ -675,6 +675,7 @@ def adamw_multi(params, grads, state_blocks, steps, m, v, m_scale=None, v_scale=
     p_c, g_c, held = _adamw_addresses(params, grads, sizes)
     _adamw_launch(device, count, p_c, g_c, array.array("q", sizes), array.array("q", state_blocks), array.array("i", steps),
                   params[0].dtype, m, v, m_scale, v_scale, lr, beta1, beta2, eps, wd)
+    torch.autograd.graph.increment_version([*params, m, v, *(t for t in (m_scale, v_scale) if t is not None)])
 
 
 _dtype_of, _ptr_of, _numel_of, _device_of = operator.attrgetter("dtype"), torch.Tensor.data_ptr, torch.Tensor.numel, \

@@ -169,7 +169,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             p_c, g_c, now = array.array("Q", bytes(8 * n)), array.array("Q", bytes(8 * n)), array.array("i", bytes(4 * n))
             # the common step: every parameter has a gradient, and all are as they were laid out
             if lib.step_list()(ps, n, _at(sizes_c), dt == torch.bfloat16, self.device.index, _at(steps), _at(p_c), _at(g_c), _at(now)):
-                calls.append((n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, None, None))
+                calls.append((n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, None, ps, None))
                 continue
             grads = list(map(_grad_of, ps))
             at = [k for k, g in enumerate(grads) if g is not None]
@@ -180,9 +180,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                     raise RuntimeError(f"MultiTensorAdamW: parameters must stay on {self.device}, where the moments are")
                 p_c, g_c, held = ops._adamw_addresses(some, [grads[k] for k in at], sizes)
                 now = array.array("i", [steps[k] + 1 for k in at])
-                calls.append((len(at), p_c, g_c, sizes_c, blocks_c, now, some[0].dtype, rates, steps, at, held))
-        for n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, at, _ in calls:
+                calls.append((len(at), p_c, g_c, sizes_c, blocks_c, now, some[0].dtype, rates, steps, at, some, held))
+        for n, p_c, g_c, sizes_c, blocks_c, now, dt, rates, steps, at, ps, _ in calls:
             ops._adamw_launch(self.device, n, p_c, g_c, sizes_c, blocks_c, now, dt, self._m, self._v, self._ms, self._vs, *rates)
+            lib.written()(ps)                        # a backward pass that saved them is to raise an error, as with torch's AdamW
             if at is None:
                 steps[:] = now
             else:
