@@ -108,6 +108,17 @@ def _call_on(device, name, *args):
             lib.call(name, *args, _stream())
 
 
+def _no_graph(who, *tensors):
+    """These operators record nothing for autograd (each has a backward call of its own): an activation that autograd follows is
+    refused, because its gradient would be missing without a word.  Weights may be Parameters as they are: their gradients
+    are what the backward call returns."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who}: records nothing for autograd, and a tensor here requires a gradient: call it under "
+                                   f"torch.no_grad() or pass detached tensors, and take the gradient from its backward call")
+
+
 def _device_index() -> int:
     return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
@@ -235,7 +246,10 @@ def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, 
     [groups, cols] of its row's group, and is normed for the next block (``pre_w``, ``pre_b``):
     x_out = x + N_post(h) * scale * gate, y = N_pre(x_out) -> (x_out, y in h's type, stats for ``res_norm_bwd`` or None).
     ``kind``: "ln" or "rms".  Groups are rows // groups rows each, or the sequences of a packed batch (``cu`` int32 [groups
-    + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (x_out may be x), zero in new ones."""
+    + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (x_out may be x), zero in new ones.
+    Nothing is recorded for autograd: x or h that require a gradient are refused where autograd is on, and the weights' gradients
+    come from ``res_norm_bwd``."""
+    _no_graph("res_norm_fwd", x, h, x_out, y)
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu,
                                                            kind)
     x_out, zx = _res_norm_out(x_out, x, f32, "res_norm_fwd")
@@ -256,6 +270,7 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
     """Backward of ``res_norm_fwd``: dy = gradient of y (h's type), dres = gradient of x_out from elsewhere (float32 or None) ->
     (dx float32, dh in h's type, {"pre_w", "pre_b", "post_w", "post_b", "scale", "gate"}: float32 gradients of what was given;
     those of a bias are there with their weight's).  ``dx`` may be dres.  Sums are formed in a fixed order."""
+    _no_graph("res_norm_bwd", dy, dres, h, x_out, dx, dh)
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu,
                                                            kind)
     if dy.shape != h.shape or dy.device != dev or tuple(stats.shape) != (4, rows) or stats.device != dev:
@@ -879,7 +894,10 @@ def token_logprobs(logits, targets=None, scale=1.0, k=0):
     """Rows of ``scale * logits`` (float32 or bfloat16 [R, V], any row pitch) -> (logp, entropy, stats, top_logp, top_idx):
     log probability of ``targets`` (int64 [R]; negative: no target, 0; V or more: NaN; None: logp is None), entropy in nats,
     the numbers the backward pass needs, and the ``k`` <= 32 most probable entries, best first, ties to the lowest index (None
-    without k).  -inf entries are masked; a row of nothing else has logp and alternatives of -inf and entropy 0."""
+    without k).  -inf entries are masked; a row of nothing else has logp and alternatives of -inf and entropy 0.  Nothing is
+    recorded for autograd: logits that require a gradient are refused where autograd is on (``token_logprobs_bwd`` is their
+    gradient)."""
+    _no_graph("token_logprobs", logits)
     R, V, ld = _logits2d(logits, "logits")
     dev, k = logits.device, int(k)
     if k < 0 or k > 32 or k > V:
@@ -899,6 +917,7 @@ def token_logprobs(logits, targets=None, scale=1.0, k=0):
 def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=1.0, out=None):
     """Gradient of sum(dlogp * logp + dentropy * entropy) with respect to ``logits``, in their type (``out``: where to write
     it, the logits themselves allowed).  ``stats`` and ``scale`` are the forward pass's; dlogp / dentropy float32 [R] or None."""
+    _no_graph("token_logprobs_bwd", logits, dlogp, dentropy, out)
     R, V, ld = _logits2d(logits, "logits")
     dev = logits.device
     if tuple(stats.shape) != (3, R) or stats.device != dev:
@@ -916,6 +935,7 @@ def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=
 def token_logprobs_fwd_bwd(logits, targets, dlogp=None, dentropy=None, scale=1.0, out=None):
     """(logp, entropy, dlogits) of ``token_logprobs`` and ``token_logprobs_bwd`` for weights that are known beforehand (a mean
     over rows, a mask): one reading of the logits where a row fits a workgroup's registers."""
+    _no_graph("token_logprobs_fwd_bwd", logits, dlogp, dentropy, out)
     R, V, ld = _logits2d(logits, "logits")
     dev = logits.device
     if dlogp is not None and targets is None:
