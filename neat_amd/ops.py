@@ -119,6 +119,13 @@ def _no_graph(who, *tensors):
                                    f"torch.no_grad() or pass detached tensors, and take the gradient from its backward call")
 
 
+def _wrote(*tensors):
+    """Outputs that the caller passed in count as written in place for autograd."""
+    given = [t for t in tensors if t is not None]
+    if given:
+        torch.autograd.graph.increment_version(given)
+
+
 def _device_index() -> int:
     return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
@@ -252,11 +259,13 @@ def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, 
     _no_graph("res_norm_fwd", x, h, x_out, y)
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu,
                                                            kind)
+    given = x_out, y
     x_out, zx = _res_norm_out(x_out, x, f32, "res_norm_fwd")
     y, zy = _res_norm_out(y, h, h.dtype, "res_norm_fwd")
     stats = torch.empty(4, rows, dtype=f32, device=dev) if save else None
     _call_on(dev, "neat_res_norm_fwd", ptrs[0], ptrs[1], dt, kd, *ptrs[2:], x_out.data_ptr(), y.data_ptr(), _ptr(stats),
              (int(zx) | 2 * int(zy)) if cu is not None else 0, rows, cols, eps)
+    _wrote(*given)
     return x_out, y, stats
 
 
@@ -277,6 +286,7 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
         raise RuntimeError("res_norm_bwd: dy must have the branch's shape and stats be the forward pass's [4, rows]")
     if dres is not None and (dres.shape != x_out.shape or dres.device != dev):
         raise RuntimeError("res_norm_bwd: dres must have the stream's shape")
+    given = dx, dh
     dx, zx = _res_norm_out(dx, x_out, f32, "res_norm_bwd")
     dh, zh = _res_norm_out(dh, h, h.dtype, "res_norm_bwd")
     names = ["pre_w", "pre_b"] + (["post_w", "post_b"] if post_w is not None else []) + (["scale"] if scale is not None else [])
@@ -289,6 +299,7 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
     _call_on(dev, "neat_res_norm_bwd", _p(dy, h.dtype, "dy"), _p(dres, f32, "dres"), hp, xp, _p(stats, f32, "stats"), dt, kd, wp, pw,
              pb, sc, gp, groups, cp, dx.data_ptr(), dh.data_ptr(), *g, ws.data_ptr(),
              (int(zx) | 2 * int(zh)) if cu is not None else 0, rows, cols)
+    _wrote(*given)
     return dx, dh, grads
 
 
@@ -919,7 +930,7 @@ def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=
     it, the logits themselves allowed).  ``stats`` and ``scale`` are the forward pass's; dlogp / dentropy float32 [R] or None."""
     _no_graph("token_logprobs_bwd", logits, dlogp, dentropy, out)
     R, V, ld = _logits2d(logits, "logits")
-    dev = logits.device
+    dev, given = logits.device, out
     if tuple(stats.shape) != (3, R) or stats.device != dev:
         raise RuntimeError(f"token_logprobs_bwd: stats must be the forward pass's float32 [3, {R}]")
     if dlogp is not None and targets is None:
@@ -929,6 +940,7 @@ def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=
     out, ldo = _lp_out(out, logits)
     _call_on(dev, "neat_token_logprobs_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, _p(stats, f32, "stats"), a, b,
              float(scale), out.data_ptr(), ldo, R, V)
+    _wrote(given)
     return out
 
 
@@ -937,7 +949,7 @@ def token_logprobs_fwd_bwd(logits, targets, dlogp=None, dentropy=None, scale=1.0
     over rows, a mask): one reading of the logits where a row fits a workgroup's registers."""
     _no_graph("token_logprobs_fwd_bwd", logits, dlogp, dentropy, out)
     R, V, ld = _logits2d(logits, "logits")
-    dev = logits.device
+    dev, given = logits.device, out
     if dlogp is not None and targets is None:
         raise RuntimeError("token_logprobs_fwd_bwd: dlogp needs targets")
     tgt, a, b = (_per_row(t, R, d, dev, n) for t, d, n in ((targets, i64, "targets"), (dlogp, f32, "dlogp"),
@@ -949,6 +961,7 @@ def token_logprobs_fwd_bwd(logits, targets, dlogp=None, dentropy=None, scale=1.0
     stats = torch.empty(3, R, dtype=f32, device=dev) if ws is not None else None
     _call_on(dev, "neat_token_logprobs_fwd_bwd", logits.data_ptr(), ld, _DTYPES[logits.dtype], tgt, a, b, float(scale),
              _ptr(logp), ent.data_ptr(), _ptr(stats), out.data_ptr(), ldo, R, V, _ptr(ws))
+    _wrote(given)
     return logp, ent, out
 
 
