@@ -370,7 +370,8 @@ int neat_token_logprobs(const void* logits, long ld, int dtype, const int64_t* t
                         float* entropy, float* stats, float* top_logp, int32_t* top_idx, int R, int V, void* ws,
                         void* stream);
 /* dlogits[r, j] = d(sum_r dlogp[r] logp[r] + dentropy[r] entropy[r]) / dlogits[r, j], of the logits' type, row pitch ld_out;
- * dlogp, dentropy f32 [R], NULL: zeros.  stats from the forward pass.  dlogits may be logits (same pitch). */
+ * dlogp, dentropy f32 [R], NULL: zeros.  stats from the forward pass.  dlogits may be logits (same pitch); where it overlaps
+ * them otherwise the call is refused. */
 int neat_token_logprobs_bwd(const void* logits, long ld, int dtype, const int64_t* target, const float* stats,
                             const float* dlogp, const float* dentropy, float scale, void* dlogits, long ld_out, int R, int V,
                             void* stream);

@@ -605,6 +605,30 @@ static int lp_check(const char* who, const void* z, long ld, int dtype, int R, i
     return NEAT_OK;
 }
 
+// whether two sets of R rows of w bytes share a byte, pitches pa and pb >= w (host)
+static bool lp_rows_meet(uintptr_t a, long pa, uintptr_t b, long pb, long R, long w) {
+    if (R <= 0 || (long)(b - a) >= (R - 1) * pa + w || (long)(a - b) >= (R - 1) * pb + w) return false;
+    if (R == 1) return true;
+    if (pa == pb) {                          // columns of one buffer, say: b's rows lie q rows and d bytes behind a's
+        const long off = (long)(b - a), q = off >= 0 ? off / pa : -((-off + pa - 1) / pa), d = off - q * pa;
+        return (d < w && -R < q && q < R) || (d + w > pa && -R < q + 1 && q + 1 < R);
+    }
+    for (long i = 0, j = 0; i < R && j < R;) {
+        const uintptr_t x = a + (uintptr_t)(i * pa), y = b + (uintptr_t)(j * pb);
+        if (x < y + (uintptr_t)w && y < x + (uintptr_t)w) return true;
+        if (x < y) ++i; else ++j;
+    }
+    return false;
+}
+// the gradient lies over the logits element by element, or apart from them
+static int lp_check_out(const char* who, const void* z, long ld, const void* dz, long ldz, int dtype, int R, int V) {
+    const long t = dtype == NEAT_F32 ? 4 : 2;
+    const bool same = z == dz && (ld == ldz || R <= 1);
+    NEAT_REQUIRE(same || !lp_rows_meet((uintptr_t)z, ld * t, (uintptr_t)dz, ldz * t, R, V * t), NEAT_ERR_ARG,
+                 "%s: the gradient overlaps the logits (it may be the logits themselves)", who);
+    return NEAT_OK;
+}
+
 }  // namespace neat
 
 using namespace neat;
@@ -648,6 +672,7 @@ extern "C" int neat_token_logprobs_bwd(const void* logits, long ld, int dtype, c
     NEAT_REQUIRE(R <= 1 || ld_out >= V, NEAT_ERR_SHAPE, "neat_token_logprobs_bwd: output row pitch %ld below V=%d", ld_out, V);
     NEAT_REQUIRE(((uintptr_t)dlogits & (dtype == NEAT_F32 ? 3 : 1)) == 0, NEAT_ERR_ARG,
                  "neat_token_logprobs_bwd: gradient is not aligned to its elements");
+    if (int rc = lp_check_out("neat_token_logprobs_bwd", logits, ld, dlogits, ld_out, dtype, R, V)) return rc;
     LpArgs g{};
     g.z = logits; g.ld = ld; g.target = target; g.stats = const_cast<float*>(stats); g.a = dlogp; g.b = dentropy; g.scale = scale;
     g.dz = dlogits; g.ldz = ld_out; g.R = R; g.V = V;
@@ -664,6 +689,7 @@ extern "C" int neat_token_logprobs_fwd_bwd(const void* logits, long ld, int dtyp
     NEAT_REQUIRE(R <= 1 || ld_out >= V, NEAT_ERR_SHAPE, "neat_token_logprobs_fwd_bwd: output row pitch %ld below V=%d", ld_out, V);
     NEAT_REQUIRE(((uintptr_t)dlogits & (dtype == NEAT_F32 ? 3 : 1)) == 0, NEAT_ERR_ARG,
                  "neat_token_logprobs_fwd_bwd: gradient is not aligned to its elements");
+    if (int rc = lp_check_out("neat_token_logprobs_fwd_bwd", logits, ld, dlogits, ld_out, dtype, R, V)) return rc;
     const LpPlan p = lp_plan(dtype == NEAT_F32 ? 4 : 8, V, true);
     if (p.S > 1) {                            // longer than a workgroup's registers: two passes
         NEAT_REQUIRE(stats, NEAT_ERR_ARG, "neat_token_logprobs_fwd_bwd: rows of %d need stats", V);

@@ -927,7 +927,7 @@ def token_logprobs(logits, targets=None, scale=1.0, k=0):
 
 def token_logprobs_bwd(logits, targets, stats, dlogp=None, dentropy=None, scale=1.0, out=None):
     """Gradient of sum(dlogp * logp + dentropy * entropy) with respect to ``logits``, in their type (``out``: where to write
-    it, the logits themselves allowed).  ``stats`` and ``scale`` are the forward pass's; dlogp / dentropy float32 [R] or None."""
+    it, the logits themselves allowed, another view that overlaps them refused).  ``stats`` and ``scale`` are the forward pass's; dlogp / dentropy float32 [R] or None."""
     _no_graph("token_logprobs_bwd", logits, dlogp, dentropy, out)
     R, V, ld = _logits2d(logits, "logits")
     dev, given = logits.device, out
