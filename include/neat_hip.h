@@ -75,8 +75,9 @@ int neat_ln_bwd_finalize_batched(const float* partial, int nblk, int cols, int c
  * h, y of `dtype` (NEAT_F32 / NEAT_BF16); weights, scale f32 [cols], gate f32 [groups, cols]; pre_b, post_w, post_b, scale,
  * gate may be NULL.  Row r belongs to group r / (rows / groups), or with cu (device i32 [groups + 1], ascending from 0, read
  * within the rows) to the g with cu[g] <= r < cu[g + 1]; rows from cu[groups] on are left as they are, or zeroed in the
- * first (zero_rest & 1: x_out, dx) and second output (& 2: y, dh).  stats f32 [4, rows] = (mean, 1/deviation) of h and of x_out for the backward pass, or NULL.
- * cols % 4 == 0, <= 4 096; f32 arrays 16-byte aligned, bf16 ones 8. */
+ * first (zero_rest & 1: x_out, dx) and second output (& 2: y, dh).  stats f32 [4, rows] = (mean, 1/deviation) of h and of x_out
+ * for the backward pass, or NULL.  An output may lie exactly over a [rows, cols] input of its element size; where it overlaps an
+ * input otherwise, or another output, the call is refused.  cols % 4 == 0, <= 4 096; f32 arrays 16-byte aligned, bf16 ones 8. */
 enum { NEAT_NORM_LAYER = 0, NEAT_NORM_RMS = 1 };
 int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const float* pre_w, const float* pre_b,
                       const float* post_w, const float* post_b, const float* scale, const float* gate, int groups,

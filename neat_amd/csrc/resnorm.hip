@@ -19,6 +19,8 @@
 // Bound by HBM: 78 848 x 512 (bf16 branch, a gate per 77 rows) forward 90 us (484 MB, 5.4 TB/s), backward 140 us (727 MB, 5.2)
 // and 9 us for the sums; 50 000 x 1 280 forward 145 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9
 // us) is the second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.3 us, a launch's latency.
+#include <initializer_list>
+
 #include "wave.h"
 
 namespace neat {
@@ -590,6 +592,24 @@ static int rn_check(const char* who, const RnArgs& a, int dtype, int kind) {
     return NEAT_OK;
 }
 
+// A byte range of an argument; row_elem: the element's size where it is [rows, cols] (such arrays may lie over each other exactly: a
+// row is read before anything is written in its place), else 0.
+struct RnSpan { const void* p; long bytes; int row_elem; };
+static bool rn_meet(const RnSpan& a, const RnSpan& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+static int rn_apart(const char* who, std::initializer_list<RnSpan> outs, std::initializer_list<RnSpan> ins) {
+    for (const RnSpan* o = outs.begin(); o != outs.end(); ++o) {
+        for (const RnSpan* q = o + 1; q != outs.end(); ++q)
+            NEAT_REQUIRE(!rn_meet(*o, *q), NEAT_ERR_ARG, "%s: two outputs overlap", who);
+        for (const RnSpan& i : ins)
+            NEAT_REQUIRE(!rn_meet(*o, i) || (o->p == i.p && o->row_elem && o->row_elem == i.row_elem), NEAT_ERR_ARG,
+                         "%s: an output overlaps an input (it may lie over an activation of its element size exactly)", who);
+    }
+    return NEAT_OK;
+}
+
 }  // namespace neat
 
 using namespace neat;
@@ -605,6 +625,11 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     if (int rc = rn_check("neat_res_norm_fwd", a, dtype, kind)) return rc;
     if (rows == 0) return NEAT_OK;
     NEAT_REQUIRE(x && h && pre_w && x_out && y, NEAT_ERR_ARG, "neat_res_norm_fwd: null pointer");
+    const int t = dtype == NEAT_F32 ? 4 : 2;
+    const long n = (long)rows * cols, w = 4L * cols;
+    if (int rc = rn_apart("neat_res_norm_fwd", {{x_out, 4 * n, 4}, {y, t * n, t}, {stats, 16L * rows, 0}},
+                          {{x, 4 * n, 4}, {h, t * n, t}, {pre_w, w, 0}, {pre_b, w, 0}, {post_w, w, 0}, {post_b, w, 0}, {scale, w, 0},
+                           {gate, w * groups, 0}, {cu, 4L * (groups + 1), 0}})) return rc;
     const int blocks = rn_fwd_blocks(rows, cols, dtype == NEAT_F32, post_w != nullptr);
     a.teams = blocks * (rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1);
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
@@ -631,6 +656,16 @@ extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* 
     NEAT_REQUIRE(pre_w && ws, NEAT_ERR_ARG, "neat_res_norm_bwd: null pointer");
     NEAT_REQUIRE((!dpost_w && !dpost_b) || post_w, NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a norm that is not there");
     NEAT_REQUIRE((!dscale || scale) && (!dgate || gate), NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a scale or gate that is not there");
+    const int t = dtype == NEAT_F32 ? 4 : 2;
+    const long n = (long)rows * cols, w = 4L * cols, ws_bytes = 4 * neat_res_norm_ws_floats(dtype, rows, cols, groups);
+    const RnSpan sc = {scale, w, 0}, gt = {gate, w * groups, 0}, at = {cu, 4L * (groups + 1), 0};
+    const RnSpan o1 = {dx, 4 * n, 4}, o2 = {dh, t * n, t}, o3 = {ws, ws_bytes, 0};
+    if (int rc = rn_apart("neat_res_norm_bwd", {o1, o2, o3},
+                          {{dy, t * n, t}, {dres, 4 * n, 4}, {h, t * n, t}, {x_out, 4 * n, 4}, {stats, 16L * rows, 0}, {pre_w, w, 0},
+                           {post_w, w, 0}, {post_b, w, 0}, sc, gt, at})) return rc;
+    // the sums are written by the second launch, which reads these
+    if (int rc = rn_apart("neat_res_norm_bwd", {{dpre_w, w, 0}, {dpre_b, w, 0}, {dpost_w, w, 0}, {dpost_b, w, 0}, {dscale, w, 0},
+                          {dgate, w * groups, 0}}, {o1, o2, o3, sc, at})) return rc;
     const bool wide = dtype == NEAT_F32;
     const int blocks = rn_bwd_blocks(rows, cols, wide);
     a.teams = blocks * (rn_bwd_wpr(cols, wide) == 1 ? RN_BWD_WAVES : 1);

@@ -253,7 +253,8 @@ def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, 
     [groups, cols] of its row's group, and is normed for the next block (``pre_w``, ``pre_b``):
     x_out = x + N_post(h) * scale * gate, y = N_pre(x_out) -> (x_out, y in h's type, stats for ``res_norm_bwd`` or None).
     ``kind``: "ln" or "rms".  Groups are rows // groups rows each, or the sequences of a packed batch (``cu`` int32 [groups
-    + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (x_out may be x), zero in new ones.
+    + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (each may be an input of its element size,
+    as x_out may be x; other overlaps are refused), zero in new ones.
     Nothing is recorded for autograd: x or h that require a gradient are refused where autograd is on, and the weights' gradients
     come from ``res_norm_bwd``."""
     _no_graph("res_norm_fwd", x, h, x_out, y)
@@ -278,7 +279,8 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
                  dh=None):
     """Backward of ``res_norm_fwd``: dy = gradient of y (h's type), dres = gradient of x_out from elsewhere (float32 or None) ->
     (dx float32, dh in h's type, {"pre_w", "pre_b", "post_w", "post_b", "scale", "gate"}: float32 gradients of what was given;
-    those of a bias are there with their weight's).  ``dx`` may be dres.  Sums are formed in a fixed order."""
+    those of a bias are there with their weight's).  ``dx`` and ``dh`` may be inputs of their element size, as dx may be dres; other
+    overlaps are refused.  Sums are formed in a fixed order."""
     _no_graph("res_norm_bwd", dy, dres, h, x_out, dx, dh)
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu,
                                                            kind)
