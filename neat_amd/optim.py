@@ -108,6 +108,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise RuntimeError(f"MultiTensorAdamW: parameters must be float32 or bfloat16, got {set(dtypes)}")
         if not all(map(torch.Tensor.is_contiguous, ps)):
             raise RuntimeError("MultiTensorAdamW: parameters must be contiguous")
+        at = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in ps if p.numel())
+        if any(b[0] < a[1] for a, b in zip(at, at[1:])):
+            raise ValueError("MultiTensorAdamW: two parameters share memory (they would be updated at once)")
         lib.step_list()                              # a missing helper is an error here, not in the first step
         self.state_bits = state_bits
         # by position in the list of all parameters: sizes, first blocks of the moments
