@@ -100,8 +100,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise ValueError("MultiTensorAdamW: empty parameter list")
         if len(set(map(id, ps))) != len(ps):
             raise ValueError("MultiTensorAdamW: a parameter is listed twice")
-        self.device = ps[0].device
-        if self.device.type != "cuda" or len(set(map(torch.Tensor.get_device, ps))) != 1:
+        if ps[0].device.type != "cuda" or len(set(map(torch.Tensor.get_device, ps))) != 1:
             raise RuntimeError("MultiTensorAdamW: parameters must be on one GPU")
         dtypes = [p.dtype for p in ps]
         if not set(dtypes) <= {torch.float32, torch.bfloat16}:
@@ -112,7 +111,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if any(b[0] < a[1] for a, b in zip(at, at[1:])):
             raise ValueError("MultiTensorAdamW: two parameters share memory (they would be updated at once)")
         lib.step_list()                              # a missing helper is an error here, not in the first step
-        self.state_bits = state_bits
+        self._lay_out(ps, state_bits)
+        self._ready = True
+
+    def _lay_out(self, ps, state_bits, buffers=None):
+        """The moments of ``ps`` (new ones, or ``buffers``), and what a step needs to know of them."""
+        self.state_bits, self.device = state_bits, ps[0].device
         # by position in the list of all parameters: sizes, first blocks of the moments
         self._params, self._numel = ps, list(map(torch.Tensor.numel, ps))
         ends = list(itertools.accumulate([-(-n // ops.ADAMW_BLOCK) for n in self._numel]))
@@ -123,21 +127,33 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             here = range(at, at + len(g["params"]))
             at = here.stop
             for dt in (torch.float32, torch.bfloat16):
-                pos = [k for k in here if dtypes[k] == dt]
+                pos = [k for k in here if ps[k].dtype == dt]
                 if pos:
                     self._lists.append([i, dt, pos, [ps[k] for k in pos], self._layout(pos), array.array("i", [0] * len(pos))])
-        dt = torch.uint8 if state_bits == 8 else torch.float32
-        self._m = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
-        self._v = torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device)
-        self._ms = torch.ones(blocks, device=self.device) if state_bits == 8 else None
-        self._vs = torch.ones(blocks, device=self.device) if state_bits == 8 else None
+        if buffers is None:
+            dt = torch.uint8 if state_bits == 8 else torch.float32
+            buffers = [torch.zeros(blocks, ops.ADAMW_BLOCK, dtype=dt, device=self.device) for _ in range(2)]
+            buffers += [torch.ones(blocks, device=self.device) for _ in range(2)] if state_bits == 8 else []
+        self._m, self._v, self._ms, self._vs = [*buffers, None, None][:4]
         # e4m3 views of the codes (the same memory)
         self.exp_avg = self._m.view(torch.float8_e4m3fn) if state_bits == 8 else self._m
         if state_bits == 8:
             self.exp_avg_root, self.exp_avg_scale, self.exp_avg_root_scale = self._v.view(torch.float8_e4m3fn), self._ms, self._vs
         else:
             self.exp_avg_sq = self._v
-        self._ready = True
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), _held=(self.state_bits, self._buffers(), self._step_counts()))
+
+    def __setstate__(self, state):
+        """For copies and pickles; torch calls it from load_state_dict too, without the moments."""
+        held = state.get("_held")
+        super().__setstate__({k: v for k, v in state.items() if k != "_held"})
+        if held is not None:
+            bits, buffers, steps = held
+            self._lay_out([p for g in self.param_groups for p in g["params"]], bits, buffers)
+            self._set_step_counts(steps)
+            self._ready = True
 
     def _layout(self, pos):
         """(sizes, the same as a C array, first blocks of the moments as a C array)."""
@@ -223,6 +239,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                       "buffers": self._buffers()}
         return d
 
+    def _set_step_counts(self, steps):
+        for _, _, pos, _, _, held in self._lists:
+            held[:] = array.array("i", [int(steps[k]) for k in pos])
+
     def load_state_dict(self, state_dict):
         st = state_dict["state"]
         if st.get("state_bits") != self.state_bits or st["numels"] != self._numel:
@@ -230,5 +250,4 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for dst, src in zip(self._buffers(), st["buffers"]):
             dst.copy_(src)
-        for _, _, pos, _, _, held in self._lists:
-            held[:] = array.array("i", [int(st["steps"][k]) for k in pos])
+        self._set_step_counts(st["steps"])
