@@ -247,7 +247,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         st = state_dict["state"]
         if st.get("state_bits") != self.state_bits or st["numels"] != self._numel:
             raise ValueError("MultiTensorAdamW: the state belongs to other parameters or another state_bits")
+        mine, given = self._buffers(), list(st["buffers"])
+        if len(st["steps"]) != len(self._numel) or [(t.shape, t.dtype) for t in given] != [(t.shape, t.dtype) for t in mine]:
+            raise ValueError("MultiTensorAdamW: the state's moments are not laid out as this optimizer's")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        for dst, src in zip(self._buffers(), st["buffers"]):
+        for dst, src in zip(mine, given):
             dst.copy_(src)
         self._set_step_counts(st["steps"])

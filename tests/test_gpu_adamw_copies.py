@@ -1,4 +1,4 @@
-"""GPU: copies and pickles of MultiTensorAdamW carry its moments and step counts."""
+"""GPU: copies and pickles of MultiTensorAdamW carry its moments and step counts, and a state that does not fit is refused whole."""
 import copy
 import io
 import pickle
@@ -58,3 +58,21 @@ def test_copies_go_on_where_the_original_was(how, bits):
     assert twin.opt.exp_avg.data_ptr() == twin.opt._m.data_ptr() != net.opt._m.data_ptr()
     with pytest.raises(RuntimeError):
         twin.opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(3, device=DEV))]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_does_not_fit_is_refused_whole(bits):
+    net, other = Net(bits), Net(bits)
+    steps(net, 1)
+    good = copy.deepcopy(net.opt.state_dict())
+    for g in other.opt.param_groups:
+        g["lr"] = 0.5
+    for spoil in (lambda s: s["buffers"].pop(), lambda s: s["steps"].pop(), lambda s: s["buffers"].__setitem__(1, s["buffers"][1][:1])):
+        bad = copy.deepcopy(good)
+        spoil(bad["state"])
+        with pytest.raises(ValueError, match="laid out"):
+            other.opt.load_state_dict(bad)
+        assert [g["lr"] for g in other.opt.param_groups] == [0.5, 0.5] and other.opt._step_counts() == [0, 0, 0]
+        assert not other.opt._m.any()
+    other.opt.load_state_dict(good)
+    assert other.opt._step_counts() == [2, 2, 1] and all(torch.equal(s, t) for s, t in zip(other.opt._buffers(), net.opt._buffers()))
