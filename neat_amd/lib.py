@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # NEAT_HIP_LIB: an alternative build of the same library (kernel A/B experiments from tools/); default: the in-tree build
@@ -118,7 +119,7 @@ def _host_lib() -> C.PyDLL:
         import torch  # noqa: F401  (the helper resolves against torch's libraries)
         path = os.path.join(_HERE, "libneat_host.so")
         if not os.path.exists(path):
-            raise RuntimeError(f"{path} not found: build it with `make -C neat_amd/csrc`")
+            raise RuntimeError(f"{path} not found: build it with `make -C neat_amd/csrc host PY={sys.executable}`")
         dll = C.PyDLL(path)
         dll.neat_host_step_list.restype, dll.neat_host_step_list.argtypes = _I, [C.py_object, _L, _P, _I, _I, _P, _P, _P, _P]
         dll.neat_host_written.restype, dll.neat_host_written.argtypes = None, [C.py_object]
