@@ -9,6 +9,9 @@
 
 #include <cstdint>
 
+// the torch and Python that this was compiled for: others lay their objects out otherwise
+extern "C" const char* neat_host_for() { return NEAT_HOST_FOR; }
+
 static bool plain(const at::Tensor& t, at::ScalarType type, int device, int64_t numel) {
     return t.defined() && t.layout() == at::kStrided && t.scalar_type() == type && t.get_device() == device && t.numel() == numel &&
            t.is_contiguous();

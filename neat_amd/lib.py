@@ -116,11 +116,19 @@ def _host_lib() -> C.PyDLL:
     """libneat_host.so (csrc/host.cpp), the package's helper that reads lists of tensors."""
     global _host
     if _host is None:
-        import torch  # noqa: F401  (the helper resolves against torch's libraries)
-        path = os.path.join(_HERE, "libneat_host.so")
+        import torch  # (the helper resolves against torch's libraries)
+        path, build = os.path.join(_HERE, "libneat_host.so"), f"`make -C neat_amd/csrc host PY={sys.executable}`"
         if not os.path.exists(path):
-            raise RuntimeError(f"{path} not found: build it with `make -C neat_amd/csrc host PY={sys.executable}`")
-        dll = C.PyDLL(path)
+            raise RuntimeError(f"{path} not found: build it with {build}")
+        here, there = "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2]), "another torch"
+        try:
+            dll = C.PyDLL(path)
+            dll.neat_host_for.restype, dll.neat_host_for.argtypes = C.c_char_p, []
+            there = dll.neat_host_for().decode()
+        except (OSError, AttributeError):                  # it does not link, or is older than this question
+            pass
+        if there != here:                                  # it reads torch's objects by their layout
+            raise RuntimeError(f"{path} was built for {there}, this is {here}: build it anew with {build}")
         dll.neat_host_step_list.restype, dll.neat_host_step_list.argtypes = _I, [C.py_object, _L, _P, _I, _I, _P, _P, _P, _P]
         dll.neat_host_written.restype, dll.neat_host_written.argtypes = None, [C.py_object]
         _host = dll
