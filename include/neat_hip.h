@@ -77,7 +77,8 @@ int neat_ln_bwd_finalize_batched(const float* partial, int nblk, int cols, int c
  * within the rows) to the g with cu[g] <= r < cu[g + 1]; rows from cu[groups] on are left as they are, or zeroed in the
  * first (zero_rest & 1: x_out, dx) and second output (& 2: y, dh).  stats f32 [4, rows] = (mean, 1/deviation) of h and of x_out
  * for the backward pass, or NULL.  An output may lie exactly over a [rows, cols] input of its element size; where it overlaps an
- * input otherwise, or another output, the call is refused.  cols % 4 == 0, <= 4 096; f32 arrays 16-byte aligned, bf16 ones 8. */
+ * input otherwise, or another output, the call is refused.  cols % 4 == 0, <= 4 096; groups <= 2^30;
+ * f32 arrays 16-byte aligned, bf16 ones 8. */
 enum { NEAT_NORM_LAYER = 0, NEAT_NORM_RMS = 1 };
 int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const float* pre_w, const float* pre_b,
                       const float* post_w, const float* post_b, const float* scale, const float* gate, int groups,
@@ -85,7 +86,8 @@ int neat_res_norm_fwd(const float* x, const void* h, int dtype, int kind, const 
                       void* stream);
 /* dy (of dtype) = gradient of y, dres f32 [rows, cols] = gradient of x_out from elsewhere (NULL: none; may be dx) -> dx f32
  * (gradient of x) and dh (of dtype), and the sums over rows dpre_w .. dscale f32 [cols], dgate f32 [groups, cols] (NULL: not
- * wanted; written, not added to).  stats, x_out from the forward pass.  ws: neat_res_norm_ws_floats floats, 16-byte aligned.
+ * wanted; written, not added to; groups x cols, cols rounded up to 64, below 2^32 where dgate is wanted).  stats, x_out from the
+ * forward pass.  ws: neat_res_norm_ws_floats floats, 16-byte aligned.
  * Sums are formed in a fixed order. */
 long neat_res_norm_ws_floats(int dtype, int rows, int cols, int groups);
 int neat_res_norm_bwd(const void* dy, const float* dres, const void* h, const float* x_out, const float* stats, int dtype, int kind,

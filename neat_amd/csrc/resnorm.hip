@@ -26,6 +26,7 @@
 namespace neat {
 
 constexpr int RN_MAX_COLS = 4096;
+constexpr int RN_MAX_GROUPS = 1 << 30;                    // team + group and the search's probes stay within an int
 constexpr int RN_FWD_WAVES = 4, RN_BWD_WAVES = 4;         // waves of a workgroup whose teams are single waves
 constexpr int RN_SUMS = 5;                                // column sums: pre_w, pre_b, post_w, post_b, scale
 
@@ -607,6 +608,7 @@ static int rn_check(const char* who, const RnArgs& a, int dtype, int kind) {
     NEAT_REQUIRE(kind == NEAT_NORM_LAYER || kind == NEAT_NORM_RMS, NEAT_ERR_ARG, "%s: kind=%d", who, kind);
     NEAT_REQUIRE(a.rows >= 0 && a.cols > 0 && a.cols % 4 == 0 && a.cols <= RN_MAX_COLS, NEAT_ERR_SHAPE,
                  "%s: rows=%d cols=%d unsupported (cols %% 4 == 0, <= %d)", who, a.rows, a.cols, RN_MAX_COLS);
+    NEAT_REQUIRE(a.groups <= RN_MAX_GROUPS, NEAT_ERR_SHAPE, "%s: groups=%d is too large", who, a.groups);
     NEAT_REQUIRE(a.groups >= 0 && (a.gate == nullptr) == (a.groups == 0), NEAT_ERR_ARG, "%s: groups=%d need a gate each", who, a.groups);
     NEAT_REQUIRE(!a.cu || a.gate, NEAT_ERR_ARG, "%s: cu without a gate", who);
     NEAT_REQUIRE(!a.gate || a.cu || a.rows % a.groups == 0, NEAT_ERR_SHAPE, "%s: rows=%d do not divide into %d groups", who,
@@ -658,7 +660,7 @@ extern "C" int neat_res_norm_fwd(const float* x, const void* h, int dtype, int k
     const long n = (long)rows * cols, w = 4L * cols;
     if (int rc = rn_apart("neat_res_norm_fwd", {{x_out, 4 * n, 4}, {y, t * n, t}, {stats, 16L * rows, 0}},
                           {{x, 4 * n, 4}, {h, t * n, t}, {pre_w, w, 0}, {pre_b, w, 0}, {post_w, w, 0}, {post_b, w, 0}, {scale, w, 0},
-                           {gate, w * groups, 0}, {cu, 4L * (groups + 1), 0}})) return rc;
+                           {gate, w * groups, 0}, {cu, 4L * groups + 4, 0}})) return rc;
     const int blocks = rn_fwd_blocks(rows, cols, dtype == NEAT_F32, post_w != nullptr);
     a.teams = blocks * (rn_fwd_wpr(cols) == 1 ? RN_FWD_WAVES : 1);
     return rn_pick<RnForward>(dtype, a, blocks, (hipStream_t)stream);
@@ -687,7 +689,7 @@ extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* 
     NEAT_REQUIRE((!dscale || scale) && (!dgate || gate), NEAT_ERR_ARG, "neat_res_norm_bwd: gradients of a scale or gate that is not there");
     const int t = dtype == NEAT_F32 ? 4 : 2;
     const long n = (long)rows * cols, w = 4L * cols, ws_bytes = 4 * neat_res_norm_ws_floats(dtype, rows, cols, groups);
-    const RnSpan sc = {scale, w, 0}, gt = {gate, w * groups, 0}, at = {cu, 4L * (groups + 1), 0};
+    const RnSpan sc = {scale, w, 0}, gt = {gate, w * groups, 0}, at = {cu, 4L * groups + 4, 0};
     const RnSpan o1 = {dx, 4 * n, 4}, o2 = {dh, t * n, t}, o3 = {ws, ws_bytes, 0};
     if (int rc = rn_apart("neat_res_norm_bwd", {o1, o2, o3},
                           {{dy, t * n, t}, {dres, 4 * n, 4}, {h, t * n, t}, {x_out, 4 * n, 4}, {stats, 16L * rows, 0}, {pre_w, w, 0},
@@ -699,15 +701,17 @@ extern "C" int neat_res_norm_bwd(const void* dy, const float* dres, const void* 
     const int blocks = rn_bwd_blocks(rows, cols, wide);
     a.teams = blocks * (rn_bwd_wpr(cols, wide) == 1 ? RN_BWD_WAVES : 1);
     a.slots = gate ? ws + (long)blocks * RN_SUMS * cols : nullptr;
-    hipStream_t s = (hipStream_t)stream;
-    if (int rc = rn_pick<RnBackward>(dtype, a, blocks, s)) return rc;
-    const RnOut o{{dpre_w, dpre_b, dpost_w, dpost_b, dscale}, dgate};
     const int cb = cdiv(cols, 64);
     // few groups with many slots each: 16 slices a group; many groups: one slice each
     const int gate_rows = groups > 0 && a.teams / groups >= 8 ? 1 : RNF_SLICES;
-    const int col_blocks = RN_SUMS * cb, gate_blocks = dgate ? cb * cdiv(groups, gate_rows) : 0;
-    hipLaunchKernelGGL(res_norm_finalize_kernel, dim3(col_blocks + gate_blocks), dim3(64 * RNF_SLICES), 0, s, a, o, blocks,
-                       col_blocks, gate_rows);
+    const long col_blocks = RN_SUMS * cb, gate_blocks = dgate ? (long)cb * cdiv(groups, gate_rows) : 0;
+    NEAT_REQUIRE((col_blocks + gate_blocks) * 64 * RNF_SLICES < 1L << 32, NEAT_ERR_SHAPE,
+                 "neat_res_norm_bwd: a gate of groups=%d x cols=%d is too large for its gradient", groups, cols);
+    hipStream_t s = (hipStream_t)stream;
+    if (int rc = rn_pick<RnBackward>(dtype, a, blocks, s)) return rc;
+    const RnOut o{{dpre_w, dpre_b, dpost_w, dpost_b, dscale}, dgate};
+    hipLaunchKernelGGL(res_norm_finalize_kernel, dim3((unsigned)(col_blocks + gate_blocks)), dim3(64 * RNF_SLICES), 0, s, a, o, blocks,
+                       (int)col_blocks, gate_rows);
     NEAT_LAUNCH_CHECK("neat_res_norm_bwd (sums)");
     return NEAT_OK;
 }
