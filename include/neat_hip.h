@@ -361,7 +361,7 @@ int neat_comm_destroy(void);
 /* ---- log probabilities of given tokens, with entropy, alternatives and gradient (the entropy and contrastive terms of
  * train_TTA.py:45-48 and zero-shot scoring of evaluation/mcq.py:92-97, for logits that are at hand) ---- */
 /* logits [R, V] of `dtype` (NEAT_F32 / NEAT_BF16), row pitch ld >= V elements, rows aligned to their elements only; z = scale *
- * logits, scale > 0.  Per row: logp[r] = log softmax(z)[target[r]] (target i64 [R]; negative: 0, there is no target; V or
+ * logits, 0 < scale <= 2^100.  Per row: logp[r] = log softmax(z)[target[r]] (target i64 [R]; negative: 0, there is no target; V or
  * more: NaN); entropy[r] = -sum p log p; stats f32 [3, R] = (max of the logits, sum exp(z - max z), entropy) for the backward
  * pass; top_logp f32 [R, k], top_idx i32 [R, k] = the k most probable, best first, ties -> lowest index, k <= 32 and <= V.
  * logp, entropy, stats may be NULL; target may be NULL with logp.  -inf logits are masked: a row of nothing else has logp =

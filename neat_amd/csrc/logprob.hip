@@ -29,6 +29,7 @@ constexpr int LP_MAX_K = 32;
 constexpr int LP_MAX_SPLIT = 64;
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 constexpr float LP_LOWEST = -160.f;          // exp2 of it is zero: keeps 0 * -inf out of the sums
+constexpr float LP_MAX_SCALE = 0x1p100f;     // and 0 * inf out of the gradient, whose factors reach 160 scale x weight
 
 struct LpArgs {
     const void* z;                           // [R, V], row pitch ld
@@ -601,7 +602,7 @@ static int lp_check(const char* who, const void* z, long ld, int dtype, int R, i
     NEAT_REQUIRE(V <= LP_MAX_SPLIT * 1024 * LP_NV * vec, NEAT_ERR_SHAPE, "%s: V=%d is above %d", who, V,
                  LP_MAX_SPLIT * 1024 * LP_NV * vec);
     NEAT_REQUIRE(((uintptr_t)z & (dtype == NEAT_F32 ? 3 : 1)) == 0, NEAT_ERR_ARG, "%s: logits are not aligned to their elements", who);
-    NEAT_REQUIRE(scale > 0.f && scale < INFINITY, NEAT_ERR_ARG, "%s: scale=%g must be positive", who, (double)scale);
+    NEAT_REQUIRE(scale > 0.f && scale <= LP_MAX_SCALE, NEAT_ERR_ARG, "%s: scale=%g must be positive, and 2^100 at most", who, (double)scale);
     return NEAT_OK;
 }
 

@@ -904,7 +904,7 @@ def _lp_out(out, logits):
 
 
 def token_logprobs(logits, targets=None, scale=1.0, k=0):
-    """Rows of ``scale * logits`` (float32 or bfloat16 [R, V], any row pitch) -> (logp, entropy, stats, top_logp, top_idx):
+    """Rows of ``scale * logits`` (float32 or bfloat16 [R, V], any row pitch; scale up to 2^100) -> (logp, entropy, stats, top_logp, top_idx):
     log probability of ``targets`` (int64 [R]; negative: no target, 0; V or more: NaN; None: logp is None), entropy in nats,
     the numbers the backward pass needs, and the ``k`` <= 32 most probable entries, best first, ties to the lowest index (None
     without k).  -inf entries are masked; a row of nothing else has logp and alternatives of -inf and entropy 0.  Nothing is
