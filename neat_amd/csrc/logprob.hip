@@ -3,7 +3,7 @@
 // With x the logits of a row, f the scale, m = max x, d_j = f (x_j - m), s = sum exp d_j, p_j = exp(d_j) / s:
 //   logp_t = d_t - log s        H = log s - sum(exp(d_j) d_j) / s      (both parts of H are >= 0: nothing cancels)
 //   d(a logp_t + b H) / dx_j = f (a (delta_jt - p_j) - b p_j (d_j - log s + H))
-// One reading of the row gives all of it: a workgroup holds its row in registers (up to 32 fp32 or 64 bf16 values a lane), so
+// One reading of the row gives all of it: a workgroup holds its row in registers (up to 32 fp32 or 64 bf16 values a lane, 64 fp32 for gradients of rows above 32 768), so
 // that neither the alternatives nor the gradient read it again.  Rows longer than a workgroup's registers are cut, the pieces'
 // (m, s, sum) and lists are joined by a second launch, and the gradient is a pass of its own.
 //
@@ -16,10 +16,11 @@
 // k-th largest of 256 to 1 024 groups' keys leaves at most k groups' elements, for which there is room.
 //
 // Bound by HBM where there are rows for all CUs: 4 928 x 49 408 bf16 with gradient 183 us (974 MB, 5.3 TB/s; the vector ALU is
-// nine tenths busy there), 2 000 x 25 014 fp32 with 10 alternatives 41 us (200 MB, 4.8 TB/s; the ranking of one row runs under the
-// loads of another).  bf16 rows with alternatives are bound by the vector ALU (10 of them: rows of 1 000 2.4, of 16 385 3.4, of
-// 49 408 3.9 TB/s).  One row of 49 408 with 5 alternatives: 8 us, half of it the exponentials of one CU.  Cutting it over 13 CUs
-// makes the sums 1 us faster and the joining launch takes 1 us with them, so rows are cut only where they do not fit.
+// nine tenths busy there, and run back to back it takes 204 us), 2 000 x 25 014 fp32 with 10 alternatives 41 us (200 MB, 4.8 TB/s;
+// the ranking of one row runs under the loads of another).  bf16 rows with alternatives are bound by the vector ALU (10 of them: rows
+// of 49 408 4.4 TB/s, of 16 385 3.8), short ones by what is paid once a row (of 1 000 2.6).  One row of 49 408 with 5 alternatives:
+// 8 us, half of it the exponentials of one CU.  Cutting it over 13 CUs makes the sums 1 us faster and the joining launch takes 1 us
+// with them, so rows are cut only where they do not fit.
 #include "wave.h"
 
 namespace neat {
@@ -535,7 +536,6 @@ static LpPlan lp_plan(int vec, int V, bool grad = false) {
     p.nv = lane / vec;
     p.threads = 64;                          // the fewest lanes that hold the row
     while (p.threads < 1024 && V > p.threads * lane) p.threads *= 2;
-    // candidates of k groups have to fit 60 KiB of LDS: k x (group's elements) x 8 B
     const long cap = (long)p.threads * lane;
     p.S = cdiv(V, cap);
     p.chunk = p.S == 1 ? V : (cdiv(V, p.S) + vec - 1) / vec * vec;

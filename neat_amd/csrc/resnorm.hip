@@ -17,8 +17,8 @@
 // slot, and a second launch adds each group's slots, and the column sums, in a fixed order: no atomics, equal bits on every run.
 //
 // Bound by HBM: 78 848 x 512 (bf16 branch, a gate per 77 rows) forward 90 us (484 MB, 5.4 TB/s), backward 140 us (727 MB, 5.2)
-// and 9 us for the sums; 50 000 x 1 280 forward 145 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 9
-// us) is the second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.3 us, a launch's latency.
+// and 9 us for the sums; 50 000 x 1 280 forward 146 us (768 MB, 5.3).  What is left of 14 851 x 768 in ragged groups (31 + 50 + 10
+// us) is the second launch and the teams' partial sums, a tenth of the traffic there.  One row: 3.1 us, a launch's latency.
 #include <initializer_list>
 
 #include "wave.h"
@@ -190,7 +190,9 @@ __device__ __forceinline__ int rn_next_group(const RnArgs& a, int g, long row, l
     return g;
 }
 
-// waves a SIMD that the forward kernel's registers are kept to (wide: fp32 activations)
+// Waves a SIMD that the forward kernel's registers are kept to (wide: fp32 activations).  Teams of four waves want a few more: 3 to 9
+// registers a lane are in scratch with two chunks (1 284 to 2 048 columns, 5.3 to 5.8 TB/s) and with four in bf16 with both norms
+// (above 3 072 columns, 5.0 TB/s)
 constexpr int rn_fwd_waves(int nch, bool wide) { return nch == 1 ? 7 : nch == 2 ? 6 : nch <= 4 - wide ? 4 : 3; }
 
 template <typename T, int WPR, int NCH, bool POST>
