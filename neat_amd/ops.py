@@ -108,15 +108,15 @@ def _call_on(device, name, *args):
             lib.call(name, *args, _stream())
 
 
-def _no_graph(who, *tensors):
+def _no_graph(who, *tensors, weights=()):
     """These operators record nothing for autograd (each has a backward call of its own): an activation that autograd follows is
-    refused, because its gradient would be missing without a word.  Weights may be Parameters as they are: their gradients
-    are what the backward call returns."""
+    refused, because its gradient would be missing without a word.  ``weights`` may be Parameters as they are (their gradients
+    are what the backward call returns), but not what a graph has computed."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{who}: records nothing for autograd, and a tensor here requires a gradient: call it under "
-                                   f"torch.no_grad() or pass detached tensors, and take the gradient from its backward call")
+        if any(t is not None and t.requires_grad for t in tensors) or \
+                any(t is not None and t.requires_grad and not t.is_leaf for t in weights):
+            raise RuntimeError(f"{who}: records nothing for autograd, and a tensor here requires a gradient: call it under "
+                               f"torch.no_grad() or pass detached tensors, and take the gradient from its backward call")
 
 
 def _wrote(*tensors):
@@ -255,9 +255,9 @@ def res_norm_fwd(x, h, pre_w, pre_b=None, post_w=None, post_b=None, scale=None, 
     ``kind``: "ln" or "rms".  Groups are rows // groups rows each, or the sequences of a packed batch (``cu`` int32 [groups
     + 1]); rows behind the last one are left alone in ``x_out`` / ``y`` that are passed in (each may be an input of its element size,
     as x_out may be x; other overlaps are refused), zero in new ones.
-    Nothing is recorded for autograd: x or h that require a gradient are refused where autograd is on, and the weights' gradients
-    come from ``res_norm_bwd``."""
-    _no_graph("res_norm_fwd", x, h, x_out, y)
+    Nothing is recorded for autograd: x or h that require a gradient, and weights or gates that a graph has computed, are refused
+    where autograd is on; the gradients come from ``res_norm_bwd``."""
+    _no_graph("res_norm_fwd", x, h, x_out, y, weights=(pre_w, pre_b, post_w, post_b, scale, gate))
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_fwd", x, h, pre_w, pre_b, post_w, post_b, scale, gate, cu,
                                                            kind)
     given = x_out, y
@@ -281,7 +281,7 @@ def res_norm_bwd(dy, dres, h, x_out, stats, pre_w, post_w=None, post_b=None, sca
     (dx float32, dh in h's type, {"pre_w", "pre_b", "post_w", "post_b", "scale", "gate"}: float32 gradients of what was given;
     those of a bias are there with their weight's).  ``dx`` and ``dh`` may be inputs of their element size, as dx may be dres; other
     overlaps are refused.  Sums are formed in a fixed order."""
-    _no_graph("res_norm_bwd", dy, dres, h, x_out, dx, dh)
+    _no_graph("res_norm_bwd", dy, dres, h, x_out, dx, dh, weights=(pre_w, post_w, post_b, scale, gate))
     rows, cols, groups, dt, kd, dev, ptrs = _res_norm_args("res_norm_bwd", x_out, h, pre_w, None, post_w, post_b, scale, gate, cu,
                                                            kind)
     if dy.shape != h.shape or dy.device != dev or tuple(stats.shape) != (4, rows) or stats.device != dev:

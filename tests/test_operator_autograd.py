@@ -43,3 +43,31 @@ def test_what_autograd_follows_is_refused(k):
         CALLS[k](False)                              # weights may be Parameters
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
         CALLS[k](True)
+
+
+def made(shape, grad):
+    t = torch.nn.Parameter(torch.ones(shape))
+    return torch.tanh(t) if grad else t                  # what a network has computed / a leaf
+
+
+FWD = [lambda g: dict(pre_w=made(8, g)), lambda g: dict(pre_w=W, pre_b=made(8, g)), lambda g: dict(pre_w=W, post_w=made(8, g)),
+       lambda g: dict(pre_w=W, post_w=W, post_b=made(8, g)), lambda g: dict(pre_w=W, scale=made(8, g)),
+       lambda g: dict(pre_w=W, gate=made((2, 8), g))]
+
+
+@pytest.mark.parametrize("k", range(len(FWD)))
+def test_weights_and_gates_that_a_graph_has_computed_are_refused(k):
+    def call(g):
+        if "pre_b" in FWD[k](g):
+            return ops.res_norm_fwd(z(False), z(False), **FWD[k](g))
+        ops.res_norm_bwd(z(False), None, z(False), z(False), torch.zeros(4, 4), **FWD[k](g))
+
+    def forward(g):
+        return ops.res_norm_fwd(z(False), z(False), **FWD[k](g))
+    for f in (call, forward):
+        with pytest.raises(RuntimeError, match="records nothing for autograd"):
+            f(True)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            f(False)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            f(True)
