@@ -112,18 +112,26 @@ def _no_graph(who, *tensors, weights=()):
     """These operators record nothing for autograd (each has a backward call of its own): an activation that autograd follows is
     refused, because its gradient would be missing without a word.  ``weights`` may be Parameters as they are (their gradients
     are what the backward call returns), but not what a graph has computed."""
-    if torch.is_grad_enabled():
-        if any(t is not None and t.requires_grad for t in tensors) or \
-                any(t is not None and t.requires_grad and not t.is_leaf for t in weights):
-            raise RuntimeError(f"{who}: records nothing for autograd, and a tensor here requires a gradient: call it under "
-                               f"torch.no_grad() or pass detached tensors, and take the gradient from its backward call")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            break
+    else:
+        for t in weights:
+            if t is not None and t.requires_grad and not t.is_leaf:
+                break
+        else:
+            return
+    raise RuntimeError(f"{who}: records nothing for autograd, and a tensor here requires a gradient: call it under torch.no_grad() or "
+                       f"pass detached tensors, and take the gradient from its backward call")
 
 
 def _wrote(*tensors):
     """Outputs that the caller passed in count as written in place for autograd."""
-    given = [t for t in tensors if t is not None]
-    if given:
-        torch.autograd.graph.increment_version(given)
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
 
 
 def _device_index() -> int:
